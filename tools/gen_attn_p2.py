@@ -76,11 +76,6 @@ S_Q2OFF = 80        # source offset of unit 2's rows of the next pass (direct Q 
 S_ODESC = 84        # s[84:87]: O descriptor actually used by the stores
 
 
-STAMPS = "--stamps" in sys.argv      # lab build: s_memtime at the top of every period -> [wave][128] dwords at %[stp]
-def stamp():
-    return ("GROUP", ["s_memtime s[88:89]", "s_waitcnt lgkmcnt(0)", "s_store_dword s88, s[90:91], 0", "s_add_u32 s90, s90, 4", "s_addc_u32 s91, s91, 0"])
-
-
 class Gen:
     def __init__(self):
         self.lines = []
@@ -395,8 +390,6 @@ def build(simple=False):
                 ins += [f"v_mul_lo_u32 {vr(TD)}, {vr(TB)}, {sr(S_OS)}", f"v_add_u32 {vr(VOFFO(k))}, {vr(TD)}, {vr(TC)}"]
     for i in ins:
         e(i)
-    if STAMPS:
-        G.emit_ins(stamp())
     # first in: K/V tile 0, the Q rows of units 0 / 1 (staging) and of unit 2 (straight to its registers); then tile 1 and the first half of tile 2
     for k in range(NPIECE):
         for i in dma_piece(KVR, VOFFR(k), "0", [f"s_add_u32 m0, {sr(S_DST)}, {1024 * k}"]):
@@ -474,8 +467,6 @@ def build(simple=False):
     # O descriptor of pass 0's (non-existent) predecessor: num_records = 0 -> every store is dropped
     e(f"s_mov_b32 {sr(S_ODESC)}, {sr(ORS)}"); e(f"s_mov_b32 {sr(S_ODESC + 1)}, {sr(ORS + 1)}"); e(f"s_mov_b32 {sr(S_ODESC + 2)}, 0"); e(f"s_mov_b32 {sr(S_ODESC + 3)}, {sr(ORS + 3)}")
     e("s_nop 7"); e("s_nop 7")
-    if STAMPS:
-        G.emit_ins(stamp())
 
     # ================= pass loop =================================================================================================
     def emit_pass(G, carry):
@@ -490,8 +481,6 @@ def build(simple=False):
                 next_u = (u + 1) % 3
                 pv_first_tile = ((j == 0 and u > 0) or (j == 1 and u == 0)) and "nozc" not in OPT     # the PV of a pass's first key tile starts its sums from 0
                 per = Period(mfma_pv(prev_u, zero_c=pv_first_tile) + mfma_qk(next_u))
-                if STAMPS:
-                    per.put([(0, stamp())])
                 per.put(carry)
                 carry = []
                 free_bank = S((u + 2) % 3, 0)           # 32 VGPRs nobody owns during period (., u)
@@ -596,8 +585,6 @@ def build(simple=False):
     e(f"s_add_u32 {sr(S_PASS)}, {sr(S_PASS)}, 1")
     e(f"s_cmp_lt_u32 {sr(S_PASS)}, {NPASS}")
     e("s_cbranch_scc1 PASS_LOOP%=")
-    if STAMPS:
-        G.emit_ins(stamp())
     # ================= epilogue: the last PV and the three drains ===============================================================
     for m in mfma_pv(2):
         e(m)
@@ -616,9 +603,6 @@ def build(simple=False):
             e(i)
         e(f"s_branch {back}")
     e("END%=:")
-    if STAMPS:
-        G.emit_ins(stamp())
-        e("s_dcache_wb")
     return G.lines
 
 
@@ -631,8 +615,6 @@ def main():
     clob = [f"v{i}" for i in range(256)] + [f"a{i}" for i in range(256)] + [f"s{i}" for i in range(40, 100)] + ["vcc", "memory"]
     with open(out, "w") as f:
         f.write("// GENERATED by tools/gen_attn_p2.py%s%s -- do not edit.  %d instructions.\n" % ("" if SEQ == 576 else f" --seq {SEQ}", " --simple" if simple else "", len(lines)))
-        if STAMPS:
-            f.write("#define UFV_VIT_P2_STAMPS 1\n")
         f.write(f"#define UFV_VIT_P2{sfx.upper()}_ASM \\\n")
         for l in lines:
             f.write('    "%s\\n\\t" \\\n' % l)

@@ -88,7 +88,7 @@ def decode(s):
     ops = [o for o in ops if o]
     R = lambda i: expand(ops[i]) if i < len(ops) else []      # noqa: E731
     dst, src = [], []
-    if op in ("s_nop", "s_barrier", "s_waitcnt", "s_dcache_wb"):
+    if op in ("s_nop", "s_barrier", "s_waitcnt"):
         pass
     elif op in ("s_branch",):
         pass
@@ -110,8 +110,6 @@ def decode(s):
         dst = R(0); src = R(1)
         if ops[0] == "exec":
             dst = ["exec"]
-    elif op in ("s_memtime", "s_store_dword"):
-        dst = R(0) if op == "s_memtime" else []; src = [] if op == "s_memtime" else R(0) + R(1)
     elif op.startswith("v_mfma"):
         dst = R(0); src = R(1) + R(2) + R(3)
     elif op == "v_permlane32_swap_b32":
@@ -217,7 +215,7 @@ def audit(ins, verbose=False):
                     st.ring_ready[k] = "ready"
             st.ring_read_since_barrier = set()
             return
-        if op in ("s_nop", "s_branch", "s_dcache_wb"):
+        if op in ("s_nop", "s_branch"):
             return
         # ---- 1. in-flight
         fl = flying(st)
