@@ -386,7 +386,7 @@ def _plain_extend(c, st, n_new):
     need = torch.where((n > 0) & fits, want - have + shared.int(), 0)
     end = torch.cumsum(need, 0)
     free = torch.argsort((refs != 0).int(), stable=True).int()                  # the free pages' ids come first, ascending
-    ok = fits & (n > 0) & (end <= (refs == 0).sum())
+    ok = fits & (n > 0) & ((need == 0) | (end <= (refs == 0).sum()))
     start = have - shared.int()
     j = torch.arange(W, device=DEV) - start[:, None]
     new = (j >= 0) & (j < need[:, None]) & ok[:, None]
