@@ -5,7 +5,7 @@
 HIPCC ?= /opt/rocm/bin/hipcc
 ARCH  ?= gfx950
 CSRC  := ufvideo_amd/csrc
-SRCS  := $(CSRC)/gemm.hip $(CSRC)/gemm256.hip $(CSRC)/gemm256_b.hip $(CSRC)/gemm256_q.hip $(CSRC)/gemm256_s.hip $(CSRC)/gemm256_r.hip $(CSRC)/gemm256_m.hip $(CSRC)/gemm256_m2.hip $(CSRC)/gemm_state.hip $(CSRC)/attn.hip $(CSRC)/ops.hip $(CSRC)/qwen2_decode.hip $(CSRC)/sam_heads.hip $(CSRC)/quant.hip $(CSRC)/loss.hip $(CSRC)/resize.hip $(CSRC)/train.hip $(CSRC)/sample.hip $(CSRC)/train_proj.hip $(CSRC)/attn_bwd.hip $(CSRC)/seg_train.hip $(CSRC)/stages.hip
+SRCS  := $(CSRC)/gemm.hip $(CSRC)/gemm256.hip $(CSRC)/gemm256_b.hip $(CSRC)/gemm256_q.hip $(CSRC)/gemm256_s.hip $(CSRC)/gemm256_r.hip $(CSRC)/gemm256_m.hip $(CSRC)/gemm256_m2.hip $(CSRC)/gemm_state.hip $(CSRC)/attn.hip $(CSRC)/ops.hip $(CSRC)/qwen2_decode.hip $(CSRC)/sam_heads.hip $(CSRC)/quant.hip $(CSRC)/loss.hip $(CSRC)/resize.hip $(CSRC)/train.hip $(CSRC)/sample.hip $(CSRC)/train_proj.hip $(CSRC)/attn_bwd.hip $(CSRC)/seg_train.hip $(CSRC)/stages.hip $(CSRC)/paged_cache.hip $(CSRC)/paged_attn.hip
 OBJS  := $(SRCS:.hip=.o)
 DEPS  := $(SRCS:.hip=.d)
 LIB   := ufvideo_amd/libufv_hip.so
@@ -13,6 +13,10 @@ EXTRA ?=
 FLAGS := --offload-arch=$(ARCH) -O3 -fPIC -std=c++17 -fvisibility=hidden -Wall -Wno-unused-function -Iinclude $(EXTRA)
 
 all: $(LIB)
+
+# the paged-cache kernels are built without packed fp32 instructions, some of whose forms have returned wrong sums on these devices now and then (hipcc makes them from
+# ordinary float code; its host pass warns that it does not know the feature).  The older sources keep their flags: their kernels agree with each other bit for bit as built.
+$(CSRC)/paged_cache.o $(CSRC)/paged_attn.o: FLAGS += -Xclang -target-feature -Xclang -packed-fp32-ops
 
 # header dependencies are the compiler's own (-MMD): a generated attention body rebuilds attn.o only
 $(CSRC)/%.o: $(CSRC)/%.hip Makefile

@@ -532,6 +532,50 @@ UFV_API int ufv_resize_bilinear_bwd(const float* dout, float* din, int N, int Hs
 /* dx = cb * (sigmoid(x) - t) + sigmoid(x) (1 - sigmoid(x)) (coef[2n] * t + coef[2n + 1]): BCE-with-logits (mean) + DICE of mask n */
 UFV_API int ufv_mask_loss_bwd(const float* x, const float* t, const float* coef, float cb, float* dx, int N, int64_t HW, void* stream);
 
+/* ---- paged KV cache (csrc/paged_cache.hip, csrc/paged_attn.hip; not in the reference, which decodes one conversation from one contiguous cache) --------------
+ * One layer's cache is pages [n_pages][page][ldkv] of bf16: a page holds `page` token rows (a power of two >= 16), a row is [Hkv*hd k | Hkv*hd v] as in the
+ * contiguous cache (a contiguous cache buffer IS a run of consecutive pages).  A batch is S slots: slot s owns row s of block_table (int32 [S, ld_table], max_pages
+ * page ids in token order, -1 = none) and kv_len[s] cached tokens (int32 [S]).  The new tokens of a step are N packed rows: slot s has rows cu_q[s] .. cu_q[s+1)-1
+ * (int32 [S+1], ascending), which are its LAST tokens (kv_len counts them already); rows at or behind cu_q[S] are left as they are.  All of these live in device
+ * memory and are read when the kernel runs: the launch arguments do not change from step to step, so a step can be recorded into a HIP graph.  Page ids are checked
+ * against n_pages on the device: a key whose page id is outside is treated as absent, a row that has no page is not stored. */
+/* rotary positions with several axes (time, height, width): table f32 [N, hd] = cos | sin of positions[axis_of[i]][n] * inv_freq[i] (the layout of ufv_rope_table:
+ * ufv_rope_kv_table, ufv_gemm_qkv_rope and the two entries below read it).  positions int64 [n_axes <= 4][N], pitch ld_pos; axis_of: hd/2 bytes in HOST memory, the axis
+ * of every frequency pair.  The angle is formed and reduced in 64 bits (ufv_rope_table forms it in 32: its HF original does). */
+UFV_API int ufv_rope_axes_table(const float* inv_freq, const int64_t* positions, int64_t ld_pos, int n_axes, const uint8_t* axis_of, int N, int hd, float* table, void* stream);
+/* rotate-half RoPE of rows of `nheads` heads by a table: y (may be x) bf16 [N, ldy]; backward != 0: the transposed rotation (gradient of the forward one) */
+UFV_API int ufv_rope_rows_table(const void* x, int64_t ldx, void* y, int64_t ldy, int N, int nheads, int hd, const float* table, int backward, void* stream);
+/* RoPE + append: row n of qkv bf16 [N, ldqkv] = [q | k | v] heads -> q_out[n] = rotated q (may be the q columns of qkv), the row's cache row = [rotated k | v].  hd % 16 == 0 */
+UFV_API int ufv_rope_kv_paged(const void* qkv, int64_t ldqkv, void* q_out, int64_t ldq, int N, int Hq, int Hkv, int hd, const float* table, void* pages, int n_pages, int page,
+                              int64_t ldkv, const int32_t* block_table, int64_t ld_table, int max_pages, const int32_t* cu_q, const int32_t* kv_len, int S, void* stream);
+/* o[n] = softmax(q k^T * scale) v of every packed row over its slot's cached tokens (causal: up to the row's own), GQA, fp32 softmax; a row that sees no key gets zeros.
+ * q, o bf16, head h at column h*hd; hd a multiple of 8 up to 256.  ws: ufv_attention_paged_ws_bytes(N, S, Hq, Hkv, hd, max_pages * page) bytes (may be 0), not shared by
+ * calls that can run at the same time. */
+UFV_API int64_t ufv_attention_paged_ws_bytes(int N, int S, int Hq, int Hkv, int hd, int max_keys);
+UFV_API int ufv_attention_paged(const void* q, int64_t ldq, void* o, int64_t ldo, int N, int Hq, int Hkv, int hd, const void* pages, int n_pages, int page, int64_t ldkv,
+                                const int32_t* block_table, int64_t ld_table, int max_pages, const int32_t* cu_q, const int32_t* kv_len, int S, float scale, int causal, void* ws,
+                                int64_t ws_bytes, void* stream);
+/* page management.  refs int32 [n_pages]: how many table entries name a page, 0 = free.  Requests are dense vectors over the slots (int32 [S]).
+ * fork: slot s with parent[s] >= 0 becomes another owner of the parent's pages (nothing is copied).  Ignored where s holds tokens or the parent is named a child itself. */
+UFV_API int ufv_kv_pages_fork(int32_t* block_table, int64_t ld_table, int max_pages, int32_t* kv_len, int S, int32_t* refs, int n_pages, int page, const int32_t* parent, void* stream);
+/* extend: room for n_new[s] further tokens of every slot, kv_len[s] += n_new[s].  Pages are the lowest free ids in slot order; a partly filled last page that is shared
+ * when the call starts is replaced by a page of its own (pairs[s] = (old, new, rows to copy), else (-1, -1, 0): ufv_kv_pages_copy moves the rows).  A slot whose share
+ * reaches past the free pages (counting the shares of all slots before it) or past its table row gets nothing; new tokens that fit its own last page need none.  granted[s] = tokens granted, cu_q int32 [S+1] = their
+ * prefix sum.  max_pages <= 2^20. */
+UFV_API int64_t ufv_kv_pages_extend_ws_bytes(int S, int n_pages);
+UFV_API int ufv_kv_pages_extend(int32_t* block_table, int64_t ld_table, int max_pages, int32_t* kv_len, int S, int32_t* refs, int n_pages, int page, const int32_t* n_new, int32_t* granted,
+                                int32_t* cu_q, int32_t* pairs, void* ws, int64_t ws_bytes, void* stream);
+/* free: slots with mask[s] != 0 give their pages back: refs - 1, table entries -1, kv_len 0 */
+UFV_API int ufv_kv_pages_free(int32_t* block_table, int64_t ld_table, int max_pages, int32_t* kv_len, int S, int32_t* refs, int n_pages, int page, const int32_t* mask, void* stream);
+/* copy: the first `rows` rows of page src to page dst in every layer of the pool (layers at a pitch of layer_bytes, rows of row_bytes); pairs int32 [n][3] = (src, dst, rows);
+ * an id outside the pool: nothing.  No page may be a dst twice or both src and dst. */
+UFV_API int ufv_kv_pages_copy(void* pool, int layers, int64_t layer_bytes, int n_pages, int page, int64_t row_bytes, const int32_t* pairs, int n, void* stream);
+/* compact: the K live pages become pages 0 .. K-1: the i-th free page below K takes the i-th live page from K on (all layers), tables and refs follow.
+ * counts int32 [2] = {K, pages moved}. */
+UFV_API int64_t ufv_kv_pages_compact_ws_bytes(int n_pages);
+UFV_API int ufv_kv_pages_compact(void* pool, int layers, int64_t layer_bytes, int64_t row_bytes, int32_t* block_table, int64_t ld_table, int max_pages, const int32_t* kv_len, int S,
+                                 int32_t* refs, int n_pages, int page, int32_t* counts, void* ws, int64_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -116,12 +116,22 @@ SIGNATURES = {
     "ufv_gemm_splitk": [_p, _i, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p],
     "ufv_attention_bwd": [_p, _l, _p, _p, _l, _p, _l, _p, _l, _p, _p, _l, _i, _i, _i, _i, _f, _p, _p],
     "ufv_attention_causal_lse": [_p, _l, _p, _l, _p, _l, _p, _l, _i, _i, _i, _i, _f, _p, _p],
+    "ufv_rope_axes_table": [_p, _p, _l, _i, _p, _i, _i, _p, _p],
+    "ufv_rope_rows_table": [_p, _l, _p, _l, _i, _i, _i, _p, _i, _p],
+    "ufv_rope_kv_paged": [_p, _l, _p, _l, _i, _i, _i, _i, _p, _p, _i, _i, _l, _p, _l, _i, _p, _p, _i, _p],
+    "ufv_attention_paged": [_p, _l, _p, _l, _i, _i, _i, _i, _p, _i, _i, _l, _p, _l, _i, _p, _p, _i, _f, _i, _p, _l, _p],
+    "ufv_kv_pages_fork": [_p, _l, _i, _p, _i, _p, _i, _i, _p, _p],
+    "ufv_kv_pages_extend": [_p, _l, _i, _p, _i, _p, _i, _i, _p, _p, _p, _p, _p, _l, _p],
+    "ufv_kv_pages_free": [_p, _l, _i, _p, _i, _p, _i, _i, _p, _p],
+    "ufv_kv_pages_copy": [_p, _i, _l, _i, _i, _l, _p, _i, _p],
+    "ufv_kv_pages_compact": [_p, _i, _l, _l, _p, _l, _i, _p, _i, _p, _i, _i, _p, _p, _l, _p],
     "ufv_attention_bwd_fused": [_p, _l, _p, _p, _l, _p, _l, _p, _l, _p, _p, _l, _p, _p, _l, _i, _i, _i, _i, _f, _p, _p],
 }
 # entry points that return a size instead of a status
 SIZE_FUNCS = {"ufv_argmax_ws_bytes": ([], _l), "ufv_attention_decode_ws_bytes": ([_i, _i, _i, _i], _i), "ufv_qwen2_decode_ws_bytes": ([_p], _l), "ufv_attention_decode_fused_ws_bytes": ([_i, _i, _i], _l), "ufv_gemm_timing_read": ([_p, _p, _i], _i), "ufv_gemm_choice": ([_i, _i, _i, _i, _i, _i], _i), "ufv_gemm_set_splitk": ([_i], _i), "ufv_gemm_qkv_rope_shape": ([_i, _i, _i, _i, _i], _i), "ufv_gemm_error_state": ([], _i),
               "ufv_qwen2_prefill_ws_bytes": ([_p, _i], _l), "ufv_vit_forward_ws_bytes": ([_p, _i], _l), "ufv_stc_forward_ws_bytes": ([_p, _i, _i], _l),
               "ufv_rmsnorm_bwd_ws_bytes": ([_i], _l), "ufv_attention_bwd_ws_bytes": ([_i, _i, _i, _i], _l), "ufv_attention_bwd_fused_ws_bytes": ([_i, _i], _l),
+              "ufv_attention_paged_ws_bytes": ([_i, _i, _i, _i, _i, _i], _l), "ufv_kv_pages_extend_ws_bytes": ([_i, _i], _l), "ufv_kv_pages_compact_ws_bytes": ([_i], _l),
               "ufv_layernorm_bwd_ws_bytes": ([_i], _l), "ufv_dwconv3x3_dw_ws_bytes": ([_i], _l), "ufv_mask_dot_bwd_ws_bytes": ([_i, _i], _l)}
 
 
