@@ -500,10 +500,9 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_paged_keys_k(PagedAttn a) {
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < NW; ++k) {
-            const float f = wm[k][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(wm[k][r] - m);
+            const float f = wm[k][r] == -INFINITY ? (wl[k][r] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(wm[k][r] - m);      // (nothing but NaN has no maximum: the NaN stays)
             sum += f * wl[k][r];
-            const f32x4 x = *reinterpret_cast<const f32x4*>(smem + k * STAGE + (r * HDP + d) * 4);
-            if (f != 0.f) o += f * x;
+            o += f * *reinterpret_cast<const f32x4*>(smem + k * STAGE + (r * HDP + d) * 4);
         }
         const int tok = (w.row0 + r) / a.G, hq = w.g * a.G + (w.row0 + r - tok * a.G);
         if (whole) {
@@ -521,36 +520,62 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_paged_keys_k(PagedAttn a) {
     }
 }
 
-// one wave per (row, q head): the parts' O with weights 2^(m_i - m), in order
-template <int UNIT>
-__global__ __launch_bounds__(256) void attn_paged_join_k(PagedAttn a) {
-    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+// The parts of one (row, q head), in a fixed order.  WPR waves work on it: lanes over quads of dims and over parts (64 / ql parts at once in a wave), so that even 64 parts are two rounds
+// of loads; the partial sums meet in LDS.  WPR = 4 from 9 parts on, else one wave, four of them to a block.
+template <int UNIT, int WPR>
+__global__ __launch_bounds__(256) void attn_paged_join_k(PagedAttn a, int ql) {
+    __shared__ float red[4][64 * 4];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t id = WPR == 4 ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
     if (id >= (int64_t)a.N * a.Hq) return;
-    const int lane = threadIdx.x & 63, n = __builtin_amdgcn_readfirstlane((int)(id / a.Hq)), hq = __builtin_amdgcn_readfirstlane((int)(id % a.Hq));
+    const int n = __builtin_amdgcn_readfirstlane((int)(id / a.Hq)), hq = __builtin_amdgcn_readfirstlane((int)(id % a.Hq));
     const int s = paged_slot_of_row(a.t.cu_q, a.t.S, n);
     if (s >= a.t.S) return;
     const int q0 = a.t.cu_q[s], q1 = a.t.cu_q[s + 1];
     if (n < q0 || n >= q1 || q0 < 0 || q1 > a.N) return;
     const int len = paged_len(a.t, s), keys = paged_part<UNIT>(len, a.nsplit) * UNIT;
     if (keys >= len) return;                                                           // one part: written already
-    const int parts = (min(paged_seen(a, len, q1 - q0, n - q0), len) + keys - 1) / keys;
+    const int parts = (min(paged_seen(a, len, q1 - q0, n - q0), len) + keys - 1) / keys;      // <= 64
     const int64_t stride = (int64_t)a.N * a.Hq, rid = (int64_t)n * a.Hq + hq;
-    const float* ml = a.part + a.nsplit * stride * a.hd + 2 * rid;
-    float m = -INFINITY;
-    for (int p = 0; p < parts; ++p) m = fmaxf(m, ml[2 * p * stride]);
-    float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int p = 0; p < parts; ++p) {
-        const float mp = ml[2 * p * stride], f = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp - m);
-        sum += f * ml[2 * p * stride + 1];
-        const float* x = a.part + (p * stride + rid) * a.hd;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lane + 64 * i < a.hd && f != 0.f) o[i] += f * x[lane + 64 * i];
+    float mp = -INFINITY, lp = 0.f;
+    if (lane < parts) {
+        const f32x2 v = *reinterpret_cast<const f32x2*>(a.part + a.nsplit * stride * a.hd + 2 * (lane * stride + rid));
+        mp = v[0];
+        lp = v[1];
     }
-    const float inv = sum > 0.f ? 1.f / sum : sum;
+    const float m = wave_max(mp);
+    const float f = mp == -INFINITY ? (lp == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(mp - m);      // (a part of nothing but NaN has no maximum: its NaN stays)
+    const float sum = wave_sum(f * lp), inv = sum > 0.f ? 1.f / sum : sum;
+    const int quad = lane & (ql - 1), sub = lane / ql, np = 64 / ql;                   // ql: lanes per part, the power of two from hd / 4 on
+    const bool mine = quad * 4 < a.hd;
+    const float* x = a.part + rid * a.hd + quad * 4;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int p0 = (WPR == 4 ? wave * np : 0); p0 < parts; p0 += 4 * WPR * np) {
+        f32x4 v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < a.hd) a.o[(int64_t)n * a.ldo + hq * a.hd + lane + 64 * i] = (bf16)(o[i] * inv);
+        for (int k = 0; k < 4; ++k) {
+            const int p = p0 + k * WPR * np + sub;
+            v[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (mine && p < parts) v[k] = *reinterpret_cast<const f32x4*>(x + p * stride * a.hd);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int p = p0 + k * WPR * np + sub;
+            const float fp = __shfl(f, p < parts ? p : 0, 64);
+            if (p < parts) o += fp * v[k];
+        }
+    }
+    for (int d = ql; d < 64; d <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], d, 64);
+    if (WPR == 4) {
+        *reinterpret_cast<f32x4*>(&red[wave][lane * 4]) = o;
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int k = 1; k < 4; ++k) o += *reinterpret_cast<const f32x4*>(&red[k][lane * 4]);
+    }
+    if (sub == 0 && mine) *reinterpret_cast<bf16x4*>(a.o + (int64_t)n * a.ldo + hq * a.hd + quad * 4) = bf16x4{(bf16)(o[0] * inv), (bf16)(o[1] * inv), (bf16)(o[2] * inv), (bf16)(o[3] * inv)};
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
@@ -579,6 +604,25 @@ Plan make_plan(int N, int S, int Hq, int Hkv, int hd, int max_keys) {
     return p;
 }
 
+template <int UNIT>
+void join(const PagedAttn& a, hipStream_t st) {
+    int ql = 2;
+    while (ql * 4 < a.hd) ql <<= 1;
+    const int64_t rows = (int64_t)a.N * a.Hq;
+    if (a.nsplit > 8) hipLaunchKernelGGL((attn_paged_join_k<UNIT, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, ql);
+    else hipLaunchKernelGGL((attn_paged_join_k<UNIT, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, ql);
+}
+
+template <int HDP, int QG>
+void launch_tile(const PagedAttn& a, const Plan& p, hipStream_t st) {
+    using C = PCfg<HDP>;
+    constexpr int smem = 2 * 64 * (C::PK + C::PV);
+    UFV_ONCE_PER_DEVICE((void)hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_tile_k<HDP, QG, 4>), hipFuncAttributeMaxDynamicSharedMemorySize, smem););
+    const int64_t total = (int64_t)p.tiles * a.Hkv * p.nsplit;
+    hipLaunchKernelGGL((attn_paged_tile_k<HDP, QG, 4>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(256), smem, st, a);
+    if (p.nsplit > 1) join<64>(a, st);
+}
+
 template <int HDP>
 int launch(const PagedAttn& a, const Plan& p, hipStream_t st) {
     using C = PCfg<HDP>;
@@ -587,13 +631,9 @@ int launch(const PagedAttn& a, const Plan& p, hipStream_t st) {
         constexpr int smem = NW * 32 * (C::PK + C::PV);
         UFV_ONCE_PER_DEVICE((void)hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_keys_k<HDP, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, smem););
         hipLaunchKernelGGL((attn_paged_keys_k<HDP, NW>), dim3(p.tiles, p.nsplit, a.Hkv), dim3(NW * 64), smem, st, a);
-        if (p.nsplit > 1) hipLaunchKernelGGL((attn_paged_join_k<32 * NW>), dim3((unsigned)(((int64_t)a.N * a.Hq + 3) / 4)), dim3(256), 0, st, a);
+        if (p.nsplit > 1) join<32 * NW>(a, st);
     } else {
-        constexpr int smem = 2 * 64 * (C::PK + C::PV);
-        UFV_ONCE_PER_DEVICE((void)hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_tile_k<HDP, 1, 4>), hipFuncAttributeMaxDynamicSharedMemorySize, smem););
-        const int64_t total = (int64_t)p.tiles * a.Hkv * p.nsplit;
-        hipLaunchKernelGGL((attn_paged_tile_k<HDP, 1, 4>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(256), smem, st, a);
-        if (p.nsplit > 1) hipLaunchKernelGGL((attn_paged_join_k<64>), dim3((unsigned)(((int64_t)a.N * a.Hq + 3) / 4)), dim3(256), 0, st, a);
+        launch_tile<HDP, 1>(a, p, st);
     }
     UFV_CHECK_LAUNCH();
     return UFV_OK;

@@ -1,5 +1,6 @@
 """Thin torch-tensor wrappers over the C ABI (include/ufv.h).  torch is used only for device
 memory and the current stream; every op below runs a hand-written HIP kernel from csrc/."""
+import functools
 import math
 
 import torch
@@ -898,39 +899,53 @@ def mask_loss_bwd(x, t, coef, cb):
 
 # ---- paged KV cache (csrc/paged_cache.hip, csrc/paged_attn.hip) ---------------------------------------------------------------------
 # One layer's pages: bf16 [n_pages, page, width], row = [Hkv*hd k | Hkv*hd v]; block_table int32 [S, max_pages], kv_len int32 [S], cu_q int32 [S + 1], refs int32 [n_pages]
-# (include/ufv.h has the conventions).  The calls run on the tensors' own device, on its current stream.
+# (include/ufv.h has the conventions).  The calls run on the tensors' own device, on its current stream.  A decode step makes a few of them per layer and the smallest kernels
+# take 2 us: the checks read every tensor's properties once, and a message is formatted only when a check fails.
 
-def _dev_call(name, dev, *args):
-    if dev.index == torch.cuda.current_device():
-        return _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
-    with torch.cuda.device(dev):
-        return _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+_BF, _F32, _I32, _I64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
 
 
-def _need(cond, msg):
-    if not cond:
-        raise _lib.UfvError(msg)
+def _on_device(di, name, *args):
+    if di == torch.cuda.current_device():
+        return _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(di))
+    with torch.cuda.device(di):
+        return _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(di))
 
 
-def _ints(dev, **named):
-    for n, t in named.items():
-        _need(t.dtype == torch.int32 and t.device == dev and (t.stride(-1) == 1 or t.shape[-1] == 1), f"{n} must be int32 on {dev} with unit stride, got {t.dtype} on {t.device}")
+def _bad(name, want, t):
+    raise _lib.UfvError(f"{name} must be {want}, got {t.dtype} {tuple(t.shape)} of strides {tuple(t.stride())} on {t.device}")
 
 
-def _rows(dev, t, cols, name):
-    _need(t.dim() == 2 and t.dtype == torch.bfloat16 and t.device == dev and t.shape[1] >= cols and t.stride(1) == 1,
-          f"{name} must be bf16 rows of at least {cols} elements on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t
+def _gpu_index(t, name):
+    di = t.get_device()
+    if di < 0:
+        raise _lib.UfvError(f"{name} must live on the GPU (the hot path has no CPU fallback)")
+    return di
 
 
-def _paged_args(pages, block_table, cu_q, kv_len, Hkv, hd):
-    _need(pages.is_cuda, "pages must live on the GPU (the hot path has no CPU fallback)")
-    _need(pages.dtype == torch.bfloat16 and pages.dim() == 3 and pages.shape[2] >= 2 * Hkv * hd and pages.stride(2) == 1 and pages.stride(0) == pages.shape[1] * pages.stride(1),
-          f"pages must be bf16 [n_pages, page, >= {2 * Hkv * hd}] with rows at one pitch, got {pages.dtype} {tuple(pages.shape)}")
+def _vec(t, n, di, name):
+    """int32 vector of n entries -> its address"""
+    if t.dtype is not _I32 or t.get_device() != di or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+        _bad(name, f"a dense int32 vector of {n} entries on cuda:{di}", t)
+    return t.data_ptr()
+
+
+def _rows(t, n, cols, di, name):
+    """bf16 rows of at least `cols` elements (n of them; None: any number) -> (address, pitch)"""
+    sh, st = t.shape, t.stride()
+    if t.dtype is not _BF or t.get_device() != di or len(sh) != 2 or sh[1] < cols or st[1] != 1 or (n is not None and sh[0] != n):
+        _bad(name, f"bf16 [{'N' if n is None else n}, >= {cols}] rows on cuda:{di}", t)
+    return t.data_ptr(), st[0]
+
+
+def _paged_args(pages, block_table, cu_q, kv_len, Hkv, hd, di):
+    sh, st, bs = pages.shape, pages.stride(), block_table.shape
+    if pages.dtype is not _BF or len(sh) != 3 or sh[2] < 2 * Hkv * hd or st[2] != 1 or st[0] != sh[1] * st[1]:
+        _bad("pages", f"bf16 [n_pages, page, >= {2 * Hkv * hd}] with all rows at one pitch", pages)
     S = kv_len.shape[0]
-    _ints(pages.device, block_table=block_table, cu_q=cu_q, kv_len=kv_len)
-    _need(block_table.dim() == 2 and block_table.shape[0] == S and cu_q.numel() == S + 1, f"block_table {tuple(block_table.shape)} / cu_q {tuple(cu_q.shape)} do not fit {S} slots")
-    return (pages.data_ptr(), pages.shape[0], pages.shape[1], pages.stride(1), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], cu_q.data_ptr(), kv_len.data_ptr(), S)
+    if block_table.dtype is not _I32 or block_table.get_device() != di or len(bs) != 2 or bs[0] != S or block_table.stride(1) != 1:
+        _bad("block_table", f"int32 [{S}, max_pages] on cuda:{di}", block_table)
+    return (pages.data_ptr(), sh[0], sh[1], st[1], block_table.data_ptr(), block_table.stride(0) if S > 1 else bs[1], bs[1], _vec(cu_q, S + 1, di, "cu_q"), _vec(kv_len, S, di, "kv_len"), S)
 
 
 def rope_axis_map(sections, interleaved=False):
@@ -945,137 +960,134 @@ def rope_axis_map(sections, interleaved=False):
 def rope_axes_table(inv_freq, positions, axis_of, out=None):
     """fp32 [N, hd]: cos | sin of positions[axis_of[i], n] * inv_freq[i] (rotary positions with up to 4 axes); positions int64 [axes, N].  Same layout as `rope_table`:
     `rope_kv`, `gemm_qkv_rope`, `rope_rows_table` and `rope_kv_paged` read it."""
-    _chk(inv_freq, torch.float32, "inv_freq")
-    dev, hd = inv_freq.device, 2 * inv_freq.shape[0]
-    _need(positions.dim() == 2 and positions.dtype == torch.int64 and positions.device == dev and (positions.stride(1) == 1 or positions.shape[1] == 1),
-          f"positions must be int64 [axes, N] on {dev}, got {positions.dtype} {tuple(positions.shape)} on {positions.device}")
-    _need(inv_freq.is_contiguous() and len(axis_of) == hd // 2 and min(axis_of) >= 0 and max(axis_of) < 256, f"axis_of must name an axis for each of the {hd // 2} pairs")
-    N = positions.shape[1]
+    di, half, sh = _gpu_index(inv_freq, "inv_freq"), inv_freq.shape[0], positions.shape
+    if inv_freq.dtype is not _F32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        _bad("inv_freq", "a dense fp32 vector", inv_freq)
+    if positions.dtype is not _I64 or len(sh) != 2 or positions.get_device() != di or (positions.stride(1) != 1 and sh[1] > 1):
+        _bad("positions", f"int64 [axes, N] on cuda:{di}", positions)
+    if len(axis_of) != half or min(axis_of) < 0 or max(axis_of) >= sh[0]:
+        raise _lib.UfvError(f"axis_of must name one of the {sh[0]} axes for each of the {half} pairs")
+    N = sh[1]
     if out is None:
-        out = torch.empty((N, hd), device=dev, dtype=torch.float32)
-    _need(out.shape == (N, hd) and out.dtype == torch.float32 and out.device == dev and out.is_contiguous(), f"out must be contiguous fp32 [{N}, {hd}] on {dev}")
+        out = torch.empty((N, 2 * half), device=inv_freq.device, dtype=_F32)
+    else:
+        _table(out, N, 2 * half, di, "out")
     if N:
-        _dev_call("ufv_rope_axes_table", dev, inv_freq.data_ptr(), positions.data_ptr(), positions.stride(0), positions.shape[0], bytes(axis_of), N, hd, out.data_ptr())
+        _on_device(di, "ufv_rope_axes_table", inv_freq.data_ptr(), positions.data_ptr(), positions.stride(0), sh[0], bytes(axis_of), N, 2 * half, out.data_ptr())
     return out
 
 
-def _rope_tab(dev, table, N, hd):
-    _need(table.dtype == torch.float32 and table.device == dev and table.shape == (N, hd) and table.is_contiguous(),
-          f"table must be contiguous fp32 [{N}, {hd}] on {dev}, got {table.dtype} {tuple(table.shape)} on {table.device}")
+def _table(t, N, hd, di, name="table"):
+    if t.dtype is not _F32 or t.get_device() != di or t.shape != (N, hd) or not t.is_contiguous():
+        _bad(name, f"contiguous fp32 [{N}, {hd}] on cuda:{di}", t)
+    return t.data_ptr()
 
 
 def rope_rows_table(x, table, col0, nheads, hd, out=None, backward=False):
     """rotate-half RoPE of the `nheads` heads at column col0 of x bf16 [N, *] by a table of `rope_table` / `rope_axes_table`: in place, or into out bf16 [N, nheads*hd].
     backward=True: the transposed rotation, i.e. the gradient with respect to the un-rotated heads."""
-    _chk(x, torch.bfloat16, "x")
-    _need(col0 >= 0, f"col0 must not be negative ({col0})")
-    _rows(x.device, x, col0 + nheads * hd, "x")
-    N = x.shape[0]
-    _rope_tab(x.device, table, N, hd)
-    src = x.data_ptr() + 2 * col0
-    if out is None:
-        dst, ldo = src, x.stride(0)
-    else:
-        _rows(x.device, out, nheads * hd, "out")
-        _need(out.shape[0] == N, f"out must have {N} rows")
-        dst, ldo = out.data_ptr(), out.stride(0)
+    if col0 < 0:
+        raise _lib.UfvError(f"col0 must not be negative ({col0})")
+    di, N = _gpu_index(x, "x"), x.shape[0]
+    src, ldx = _rows(x, None, col0 + nheads * hd, di, "x")
+    src += 2 * col0
+    dst, ldo = (src, ldx) if out is None else _rows(out, N, nheads * hd, di, "out")
+    tab = _table(table, N, hd, di)
     if N:
-        _dev_call("ufv_rope_rows_table", x.device, src, x.stride(0), dst, ldo, N, nheads, hd, table.data_ptr(), int(backward))
+        _on_device(di, "ufv_rope_rows_table", src, ldx, dst, ldo, N, nheads, hd, tab, int(backward))
     return x if out is None else out
 
 
 def rope_kv_paged(qkv, table, Hq, Hkv, hd, pages, block_table, cu_q, kv_len, q_out=None):
     """RoPE of the packed new tokens' q and k heads and append of their k / v rows to the pages (the paged form of `rope_kv`).  qkv bf16 [N, (Hq + 2 Hkv)*hd]; kv_len
     counts the new tokens already (kv_pages_extend).  Returns the rotated q: the q columns of qkv, or q_out bf16 [N, Hq*hd].  Rows behind cu_q[S] stay as they are."""
-    pa = _paged_args(pages, block_table, cu_q, kv_len, Hkv, hd)
-    dev = pages.device
-    _rows(dev, qkv, (Hq + 2 * Hkv) * hd, "qkv")
+    di = _gpu_index(pages, "pages")
+    pa = _paged_args(pages, block_table, cu_q, kv_len, Hkv, hd, di)
     N = qkv.shape[0]
-    _rope_tab(dev, table, N, hd)
-    if q_out is None:
-        q_out = qkv[:, :Hq * hd]
-    _rows(dev, q_out, Hq * hd, "q_out")
-    _need(q_out.shape[0] == N, f"q_out must have {N} rows")
+    src, ldx = _rows(qkv, None, (Hq + 2 * Hkv) * hd, di, "qkv")
+    dst, ldo = (src, ldx) if q_out is None else _rows(q_out, N, Hq * hd, di, "q_out")
+    tab = _table(table, N, hd, di)
     if N:
-        _dev_call("ufv_rope_kv_paged", dev, qkv.data_ptr(), qkv.stride(0), q_out.data_ptr(), q_out.stride(0), N, Hq, Hkv, hd, table.data_ptr(), *pa)
-    return q_out
+        _on_device(di, "ufv_rope_kv_paged", src, ldx, dst, ldo, N, Hq, Hkv, hd, tab, *pa)
+    return qkv[:, :Hq * hd] if q_out is None else q_out
+
+
+@functools.lru_cache(maxsize=256)
+def _attention_paged_ws(N, S, Hq, Hkv, hd, max_keys):
+    return int(_lib.load().ufv_attention_paged_ws_bytes(N, S, Hq, Hkv, hd, max_keys))
 
 
 def attention_paged(q, pages, block_table, cu_q, kv_len, Hq, Hkv, hd, scale=None, causal=True, out=None):
     """Attention of the packed new tokens (q bf16 [N, Hq*hd], slot s has rows cu_q[s] .. cu_q[s+1]) over their slots' cached tokens: a chunk of a prompt, a decode step of
     many conversations, or both in one batch.  causal: a row sees the cached tokens up to its own.  A row that sees none gets zeros, rows behind cu_q[S] stay as they are."""
-    pa = _paged_args(pages, block_table, cu_q, kv_len, Hkv, hd)
-    dev = pages.device
-    _rows(dev, q, Hq * hd, "q")
+    di = _gpu_index(pages, "pages")
+    pa = _paged_args(pages, block_table, cu_q, kv_len, Hkv, hd, di)
     N = q.shape[0]
+    src, ldq = _rows(q, None, Hq * hd, di, "q")
     if out is None:
-        out = torch.empty((N, Hq * hd), device=dev, dtype=torch.bfloat16)
-    _rows(dev, out, Hq * hd, "out")
-    _need(out.shape[0] == N, f"out must have {N} rows")
+        out = torch.empty((N, Hq * hd), device=q.device, dtype=_BF)
+    dst, ldo = _rows(out, N, Hq * hd, di, "out")
     if N:
-        nbytes = _lib.load().ufv_attention_paged_ws_bytes(N, pa[9], Hq, Hkv, hd, min(pa[6] * pa[2], 0x7fffffff))
-        ws = torch.empty((nbytes,), device=dev, dtype=torch.uint8) if nbytes > 0 else None       # the caching allocator's: private to this call, also inside a captured graph
-        _dev_call("ufv_attention_paged", dev, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), N, Hq, Hkv, hd, *pa, hd ** -0.5 if scale is None else float(scale),
-                  int(causal), _ptr(ws), nbytes)
+        nbytes = _attention_paged_ws(N, pa[9], Hq, Hkv, hd, min(pa[6] * pa[2], 0x7fffffff))
+        ws = torch.empty((nbytes,), device=q.device, dtype=torch.uint8) if nbytes > 0 else None       # the caching allocator's: private to this call, also inside a captured graph
+        _on_device(di, "ufv_attention_paged", src, ldq, dst, ldo, N, Hq, Hkv, hd, *pa, hd ** -0.5 if scale is None else scale, int(causal), 0 if ws is None else ws.data_ptr(), nbytes)
     return out
 
 
-def _table_args(block_table, kv_len, refs, page, **vectors):
-    _chk(block_table, torch.int32, "block_table")
-    S = kv_len.shape[0]
-    _ints(block_table.device, block_table=block_table, kv_len=kv_len, refs=refs, **vectors)
-    _need(block_table.dim() == 2 and block_table.shape[0] == S and refs.dim() == 1, f"block_table {tuple(block_table.shape)} does not fit {S} slots")
-    for n, t in vectors.items():
-        _need(t.shape == (S,), f"{n} must have one entry per slot ({S}), got {tuple(t.shape)}")
-    return (block_table.data_ptr(), block_table.stride(0), block_table.shape[1], kv_len.data_ptr(), S, refs.data_ptr(), refs.shape[0], page)
+def _table_args(block_table, kv_len, refs, page):
+    di, bs, S = _gpu_index(block_table, "block_table"), block_table.shape, kv_len.shape[0]
+    if block_table.dtype is not _I32 or len(bs) != 2 or bs[0] != S or block_table.stride(1) != 1:
+        _bad("block_table", f"int32 [{S}, max_pages]", block_table)
+    P = refs.shape[0]
+    return di, S, P, (block_table.data_ptr(), block_table.stride(0) if S > 1 else bs[1], bs[1], _vec(kv_len, S, di, "kv_len"), S, _vec(refs, P, di, "refs"), P, page)
 
 
 def kv_pages_fork(block_table, kv_len, refs, parent, page):
     """slot s with parent[s] >= 0 (int32 [S]) becomes another owner of the parent's pages; a slot that holds tokens, or whose parent is named a child itself, is left as it is"""
-    _dev_call("ufv_kv_pages_fork", block_table.device, *_table_args(block_table, kv_len, refs, page, parent=parent), parent.data_ptr())
+    di, S, _, a = _table_args(block_table, kv_len, refs, page)
+    _on_device(di, "ufv_kv_pages_fork", *a, _vec(parent, S, di, "parent"))
 
 
 def kv_pages_extend(block_table, kv_len, refs, n_new, page):
     """room for n_new[s] (int32 [S]) further tokens of every slot -> (granted int32 [S], cu_q int32 [S + 1], pairs int32 [S, 3]); include/ufv.h ufv_kv_pages_extend.
     `kv_pages_copy(pool, pairs)` must follow before the new tokens are appended: pairs name the shared last pages that slots got a page of their own for."""
-    a = _table_args(block_table, kv_len, refs, page, n_new=n_new)
-    dev, S = block_table.device, a[4]
-    out = torch.empty((5 * S + 1,), device=dev, dtype=torch.int32)
-    granted, pairs, cu_q = out[:S], out[S:4 * S].view(S, 3), out[4 * S:]
-    ws = torch.empty((_lib.load().ufv_kv_pages_extend_ws_bytes(S, a[6]),), device=dev, dtype=torch.uint8)
-    _dev_call("ufv_kv_pages_extend", dev, *a, n_new.data_ptr(), granted.data_ptr(), cu_q.data_ptr(), pairs.data_ptr(), ws.data_ptr(), ws.numel())
-    return granted, cu_q, pairs
+    di, S, P, a = _table_args(block_table, kv_len, refs, page)
+    nn = _vec(n_new, S, di, "n_new")
+    granted, cu_q, pairs, ws = torch.empty((8 * S + 1 + P,), device=block_table.device, dtype=_I32).split((S, S + 1, 3 * S, 3 * S + P))
+    _on_device(di, "ufv_kv_pages_extend", *a, nn, granted.data_ptr(), cu_q.data_ptr(), pairs.data_ptr(), ws.data_ptr(), 4 * (3 * S + P))
+    return granted, cu_q, pairs.view(S, 3)
 
 
 def kv_pages_free(block_table, kv_len, refs, mask, page):
     """the slots with mask[s] != 0 (int32 [S]) give their pages back"""
-    _dev_call("ufv_kv_pages_free", block_table.device, *_table_args(block_table, kv_len, refs, page, mask=mask), mask.data_ptr())
+    di, S, _, a = _table_args(block_table, kv_len, refs, page)
+    _on_device(di, "ufv_kv_pages_free", *a, _vec(mask, S, di, "mask"))
 
 
 def _pool_args(pool):
-    _chk(pool, torch.bfloat16, "pool")
-    _need(pool.dim() == 4 and pool[0].is_contiguous(), f"pool must be bf16 [layers, n_pages, page, width] with contiguous layers, got {tuple(pool.shape)}")
-    L, P, page, width = pool.shape
-    return pool.data_ptr(), L, 2 * pool.stride(0), P, page, 2 * width
+    di, sh, st = _gpu_index(pool, "pool"), pool.shape, pool.stride()
+    if pool.dtype is not _BF or len(sh) != 4 or st[3] != 1 or st[2] != sh[3] or st[1] != sh[2] * sh[3]:
+        _bad("pool", "bf16 [layers, n_pages, page, width] with contiguous layers", pool)
+    return di, pool.data_ptr(), sh[0], 2 * st[0], sh[1], sh[2], 2 * sh[3]
 
 
 def kv_pages_copy(pool, pairs):
     """the first `rows` rows of page src to page dst in every layer of pool bf16 [layers, n_pages, page, width]; pairs int32 [n, 3] = (src, dst, rows), ids outside the pool:
     nothing.  No page may be dst twice, or src and dst."""
-    a = _pool_args(pool)
-    _ints(pool.device, pairs=pairs)
-    _need(pairs.dim() == 2 and pairs.shape[1] == 3 and pairs.is_contiguous(), f"pairs must be int32 [n, 3], got {tuple(pairs.shape)}")
-    for i in range(0, pairs.shape[0], 65535):
-        part = pairs[i:i + 65535]
-        _dev_call("ufv_kv_pages_copy", pool.device, *a, part.data_ptr(), part.shape[0])
+    di, *a = _pool_args(pool)
+    sh = pairs.shape
+    if pairs.dtype is not _I32 or pairs.get_device() != di or len(sh) != 2 or sh[1] != 3 or not pairs.is_contiguous():
+        _bad("pairs", f"int32 [n, 3] on cuda:{di}", pairs)
+    for i in range(0, sh[0], 65535):
+        _on_device(di, "ufv_kv_pages_copy", *a, pairs.data_ptr() + 12 * i, min(sh[0] - i, 65535))
 
 
 def kv_pages_compact(pool, block_table, kv_len, refs):
     """the live pages become the lowest ids (least number of page copies, all layers of pool), tables and refs follow -> counts int32 [2] = (live pages, pages moved)"""
-    ptr, L, lb, P, page, rb = _pool_args(pool)
-    a = _table_args(block_table, kv_len, refs, page)
-    _need(pool.device == block_table.device and refs.shape[0] == P, f"refs must have one entry per page ({P})")
-    counts = torch.empty((2,), device=pool.device, dtype=torch.int32)
-    ws = torch.empty((_lib.load().ufv_kv_pages_compact_ws_bytes(P),), device=pool.device, dtype=torch.uint8)
-    _dev_call("ufv_kv_pages_compact", pool.device, ptr, L, lb, rb, *a, counts.data_ptr(), ws.data_ptr(), ws.numel())
+    dp, ptr, L, lb, NP, page, rb = _pool_args(pool)
+    di, S, P, a = _table_args(block_table, kv_len, refs, page)
+    if dp != di or NP != P:
+        raise _lib.UfvError(f"refs must have one entry for each of the pool's {NP} pages ({P}), tables and pool live on one device")
+    counts, ws = torch.empty((2 + 3 * P,), device=pool.device, dtype=_I32).split((2, 3 * P))
+    _on_device(di, "ufv_kv_pages_compact", ptr, L, lb, rb, *a, counts.data_ptr(), ws.data_ptr(), 12 * P)
     return counts
