@@ -18,6 +18,7 @@ namespace {
 typedef __attribute__((ext_vector_type(2))) float f32x2;
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
 
+
 struct PagedAttn {
     const bf16 *q, *pages;
     bf16* o;
@@ -25,9 +26,18 @@ struct PagedAttn {
     PagedTable t;
     int N, Hq, Hkv, G, hd, causal;
     float sl2;              // scale * log2(e)
-    int nsplit, tiles;      // key parts (upper bound), row tiles (upper bound)
-    float* part;            // [nsplit][N * Hq][hd] un-normalised O, then [nsplit][N * Hq][2] max | sum; nullptr: nsplit == 1
+    int nsplit, tiles;      // key parts (keys kernel: upper bound) or workers (tile kernel), row tiles (upper bound)
+    float* part;            // keys kernel: [nsplit][N * Hq][hd] un-normalised O, then [nsplit][N * Hq][2] max | sum.  Tile kernel: PShare, PItem [Hkv][tiles], parts (tile_part)
 };
+
+// tile kernel: what the join needs to know, written by the kernel itself
+struct PShare { int64_t steps; int64_t pad; };                    // key steps of a worker's share
+struct PItem { int64_t start; int64_t cost; };                    // first step of a (kv head, row tile) in the order of all steps, its number of steps
+template <int R>
+__device__ __forceinline__ float* tile_part(const PagedAttn& a, int64_t worker, int which) {
+    char* base = reinterpret_cast<char*>(a.part) + 16 + 16 * (int64_t)a.Hkv * a.tiles;
+    return reinterpret_cast<float*>(base) + (worker * 2 + which) * ((int64_t)R * (a.hd + 2));       // R rows of hd, then R pairs (max, sum)
+}
 
 // what a block works on: all of it wave-uniform
 struct PagedTile {
@@ -39,12 +49,15 @@ struct PagedTile {
 // Row tiles are numbered over the batch without the host knowing the lengths: slot s may use the numbers from floor(cu_q[s] * G / R) + s on; the next slot's first number is
 // never less than what slot s needs (ceil(n G / R)).  Numbers without rows leave at once.
 template <int R>
+__device__ __forceinline__ int paged_first_tile(const PagedAttn& a, int s) { return (int)((int64_t)a.t.cu_q[s] * a.G / R) + s; }
+
+template <int R>
 __device__ __forceinline__ bool paged_tile(const PagedAttn& a, int tile, PagedTile& w) {
     const int lane = threadIdx.x & 63;
     int b = 0;
     for (int s0 = 0; s0 < a.t.S; s0 += 64) {
         const int s = s0 + lane;
-        const bool mine = s < a.t.S && (int)((int64_t)a.t.cu_q[s] * a.G / R) + s <= tile;
+        const bool mine = s < a.t.S && paged_first_tile<R>(a, s) <= tile;
         const int c = __popcll(__ballot(mine));
         b += c;
         if (c < 64) break;
@@ -109,12 +122,18 @@ struct PState {
     }
 };
 
-template <int HDP, int QG, int NH>
-__device__ __forceinline__ void paged_step(const char* kb, const char* vb, const bf16x8 (&qf)[QG][HDP / 16], PState<HDP, QG>& st, float sl2, bool hide, const int (&vis)[QG], unsigned groups) {
+// at_qk(i) / at_pv(i, n) run behind the i-th product of S^T / behind the i-th of the n products of O^T: the loads and LDS writes of the next step go there, a few at a time -- issued in
+// one go they hold the wave for 1300 + 700 of the 4900 cycles of a step (the memory pipe takes one 1 KB load in 16 cycles), behind the products they cost nothing.
+template <int HDP, int QG, int NH, class FQ, class FB, class FP>
+__device__ __forceinline__ void paged_step(const char* kb, const char* vb, const bf16x8 (&qf)[QG][HDP / 16], PState<HDP, QG>& st, float sl2, bool hide, const int (&vis)[QG], unsigned groups,
+                                           FQ&& at_qk, FB&& before_pv, FP&& at_pv) {
     using C = PCfg<HDP>;
     const int lane = threadIdx.x & 63, h = lane >> 5, l31 = lane & 31;
     const int k_off = l31 * C::PK + h * 16;
     const int v_off = (4 * h + ((lane & 15) >> 2)) * C::PV + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+    // Left to itself the compiler puts every LDS read right in front of the matrix instruction that needs it and waits out the LDS latency 32 times a step.  The order below is pinned
+    // (sched_barrier): AHEAD fragments are in flight at any time, the V reads start before the exponentials, and the second half's exponentials go between the first half's products.
+    constexpr int AHEAD = 4, NR = C::KS * NH, PRE = AHEAD < NR ? AHEAD : NR;
     f32x16 s[QG][NH];
 #pragma unroll
     for (int q = 0; q < QG; ++q)
@@ -122,26 +141,33 @@ __device__ __forceinline__ void paged_step(const char* kb, const char* vb, const
         for (int hh = 0; hh < NH; ++hh)
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[q][hh][r] = 0.f;
+    {
+        bf16x8 kf[PRE];
+        auto read = [&](int i) { return *reinterpret_cast<const bf16x8*>(kb + (i % NH) * 32 * C::PK + k_off + (i / NH) * 32); };
 #pragma unroll
-    for (int ks = 0; ks < C::KS; ++ks)
+        for (int i = 0; i < PRE; ++i) kf[i] = read(i);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int hh = 0; hh < NH; ++hh) {
-            const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kb + hh * 32 * C::PK + k_off + ks * 32);
+        for (int i = 0; i < NR; ++i) {
 #pragma unroll
-            for (int q = 0; q < QG; ++q) s[q][hh] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[q][ks], s[q][hh], 0, 0, 0);
+            for (int q = 0; q < QG; ++q) s[q][i % NH] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i % PRE], qf[q][i / NH], s[q][i % NH], 0, 0, 0);
+            if (i + PRE < NR) kf[i % PRE] = read(i + PRE);
+            at_qk(i, NR);
+            __builtin_amdgcn_sched_barrier(0);
         }
+    }
     if (hide) {
 #pragma unroll
-        for (int q = 0; q < QG; ++q)
+        for (int q = 0; q < QG; ++q) {
+            const int lim = vis[q] - 4 * h;
 #pragma unroll
             for (int hh = 0; hh < NH; ++hh)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int j = hh * 32 + (r & 3) + 8 * (r >> 2) + 4 * h;
-                    s[q][hh][r] = j < vis[q] && ((groups >> (2 * hh + (r >> 3))) & 1) ? s[q][hh][r] : -INFINITY;
-                }
+                for (int r = 0; r < 16; ++r)                          // key hh * 32 + (r & 3) + 8 (r >> 2) + 4 h
+                    s[q][hh][r] = hh * 32 + (r & 3) + 8 * (r >> 2) < lim && ((groups >> (2 * hh + (r >> 3))) & 1) ? s[q][hh][r] : -INFINITY;
+        }
     }
-    bf16x8 pf[QG][2 * NH];
+    float msub[QG];
 #pragma unroll
     for (int q = 0; q < QG; ++q) {
         float tmax = s[q][0][0];
@@ -161,32 +187,54 @@ __device__ __forceinline__ void paged_step(const char* kb, const char* vb, const
                 for (int r = 0; r < 16; ++r) st.o[q][i][r] *= alpha;
             st.m[q] = mnew;
         }
-        const float msub = st.m[q] == -INFINITY ? 0.f : st.m[q];
-        float sum = 0.f;
+        msub[q] = st.m[q] == -INFINITY ? 0.f : st.m[q];
+    }
+    before_pv();
+    constexpr int NM = 2 * C::DT, NV = NM * NH, PREV = AHEAD < NV ? AHEAD : NV, EPM = (16 + NM - 1) / NM;      // products of a half, of the step; elements per product
+    bf16x4 vf[PREV][2];
+    auto readv = [&](int i, int u) {                       // product i: keys 16 (i / DT) .., dims 32 (i % DT) ..
+        const char* vp = vb + 16 * (i / C::DT) * C::PV + v_off + (i % C::DT) * 64 + u * 8 * C::PV;
+        return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((bf16x4 __attribute__((address_space(3)))*)(vp));
+    };
 #pragma unroll
-        for (int hh = 0; hh < NH; ++hh) {
-            float p[16];
+    for (int i = 0; i < PREV; ++i) { vf[i][0] = readv(i, 0); vf[i][1] = readv(i, 1); }
+    __builtin_amdgcn_sched_barrier(0);
+    float sum[QG];
+    auto exps = [&](int hh, int r0, int r1) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[q][hh][r], sl2, -msub));
-                sum += p[r];
+        for (int q = 0; q < QG; ++q)
+#pragma unroll
+            for (int r = r0; r < r1; ++r) {
+                s[q][hh][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[q][hh][r], sl2, -msub[q]));
+                sum[q] = hh == 0 && r == 0 ? s[q][hh][r] : sum[q] + s[q][hh][r];
             }
-            pf[q][2 * hh] = pack8(p);
-            pf[q][2 * hh + 1] = pack8(p + 8);
+    };
+    exps(0, 0, 16);
+    bf16x8 pf[QG][2];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if (i % NM == 0) {
+#pragma unroll
+            for (int q = 0; q < QG; ++q)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float p[8];
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) p[r] = s[q][i / NM][8 * c + r];
+                    pf[q][c] = pack8(p);
+                }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        st.l[q] += sum;
+        const bf16x8 v = __builtin_shufflevector(vf[i % PREV][0], vf[i % PREV][1], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+        for (int q = 0; q < QG; ++q) st.o[q][i % C::DT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, pf[q][(i % NM) / C::DT], st.o[q][i % C::DT], 0, 0, 0);
+        if (i + PREV < NV) { vf[i % PREV][0] = readv(i + PREV, 0); vf[i % PREV][1] = readv(i + PREV, 1); }
+        at_pv(i, NV);
+        if (NH == 2 && i < NM) exps(1, EPM * i < 16 ? EPM * i : 16, EPM * (i + 1) < 16 ? EPM * (i + 1) : 16);
+        __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int dt = 0; dt < C::DT; ++dt)
-#pragma unroll
-        for (int c = 0; c < 2 * NH; ++c) {
-            const char* vp = vb + 16 * c * C::PV + v_off + dt * 64;
-            const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((bf16x4 __attribute__((address_space(3)))*)(vp));
-            const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((bf16x4 __attribute__((address_space(3)))*)(vp + 8 * C::PV));
-            const bf16x8 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-            for (int q = 0; q < QG; ++q) st.o[q][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[q][c], st.o[q][dt], 0, 0, 0);
-        }
+    for (int q = 0; q < QG; ++q) st.l[q] += sum[q];
 }
 
 // A key that a row does not see must not reach it even when its V row holds Inf or NaN (0 * Inf in the matrix product): among the new tokens of a causal chunk -- the only keys
@@ -247,53 +295,57 @@ __device__ __forceinline__ void paged_load_q(const PagedAttn& a, const PagedTile
 }
 
 // Staging of NG groups of 16 keys by NWS waves, cache -> registers -> LDS.  A wave load covers RPW <= 16 rows that start at a multiple of RPW, and a page holds whole groups of 16
-// tokens: the page is the same for the whole load, its id a scalar, and the lane's part of the address does not change.  Lanes whose chunk lies behind hd (padded head dims) fetch
-// chunk 0: their K meets zeros in Q, their V columns are not stored.
+// tokens: the page is the same for the whole load and its address a scalar; the lane's part of the address does not change.  Lanes whose chunk lies behind hd (padded head dims) fetch
+// chunk 0: their K meets zeros in Q, their V columns are not stored.  The ids come by a vector load (lane i: group i) behind the rows of the step before: a scalar load would share its
+// counter with the LDS reads and be waited out before the next barrier, every step.
 template <int HDP, int NG, int NWS>
 struct PStage {
     using C = PCfg<HDP>;
     static constexpr int PASS = NWS * C::RPW, RPT = 16 * NG / PASS;
     static_assert(RPT >= 1 && RPT * PASS == 16 * NG, "whole passes");
     u32x4 k[RPT], v[RPT];
-    int id[NG];             // page ids of the next step's groups, -1 behind the last token
+    int idv;                // lane i < NG: page id of the next step's group i
+    int id[NG];             // the same as scalars, -1 where there is no key or no such page
 
-    __device__ __forceinline__ void ids(const PagedAttn& a, const PagedTile& w, int step) {
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            const int64_t j = ((int64_t)step * NG + i) * 16;
-            id[i] = j < w.len ? a.t.table[(int64_t)w.s * a.t.ld + (int)(j >> a.t.sh)] : -1;
-        }
+    __device__ __forceinline__ void load_ids(const PagedAttn& a, const PagedTile& w, int step) {
+        const int64_t j = ((int64_t)step * NG + (threadIdx.x & (NG - 1))) * 16;
+        const int i = min((int)(j >> a.t.sh), a.t.width - 1);
+        idv = a.t.table[(int64_t)w.s * a.t.ld + i];
     }
-    __device__ __forceinline__ unsigned valid(const PagedAttn& a) const {
+    // scalars of the ids loaded for `step`; bit i: group i has keys
+    __device__ __forceinline__ unsigned take_ids(const PagedAttn& a, const PagedTile& w, int step) {
         unsigned ok = 0;
 #pragma unroll
-        for (int i = 0; i < NG; ++i) ok |= (unsigned)id[i] < (unsigned)a.t.n_pages ? 1u << i : 0u;
+        for (int i = 0; i < NG; ++i) {
+            id[i] = __builtin_amdgcn_readlane(idv, i);
+            const bool there = ((int64_t)step * NG + i) * 16 < w.len && (unsigned)id[i] < (unsigned)a.t.n_pages;
+            id[i] = there ? id[i] : -1;
+            ok |= there ? 1u << i : 0u;
+        }
         return ok;
     }
-    // lane_off: element offset of the lane's row and chunk inside a load; wave: the wave's place among the NWS
-    __device__ __forceinline__ void fetch(const PagedAttn& a, const PagedTile& w, int step, unsigned ok, int64_t lane_off, int srow, int wave) {
-        const bool all = ok == (1u << NG) - 1 && ((int64_t)step + 1) * NG * 16 <= w.len;
-        const bf16* base = a.pages + w.g * a.hd;
-        const int64_t vo = (int64_t)a.Hkv * a.hd;
+    // load l (of 2 RPT: K rows, then V rows) of the step whose ids were taken.  It is never conditional: where there is no page it reads page 0, behind the last token whatever the page
+    // holds; blank() puts zeros there before the rows are parked.  lane_off: byte offset of the lane's row and chunk inside a load; wave: the wave's place among the NWS
+    __device__ __forceinline__ void fetch(const PagedAttn& a, const PagedTile& w, int step, int l, unsigned lane_off, int wave) {
+        const int i = l % RPT, row = i * PASS + wave * C::RPW, j = step * NG * 16 + row;
+        int page = id[(i * PASS) >> 4];
+        if (PASS > 16)
+#pragma unroll
+            for (int x = 1; x < PASS / 16; ++x) page = (wave * C::RPW) >> 4 == x ? id[((i * PASS) >> 4) + x] : page;
+        page = max(page, 0);
+        const char* base = reinterpret_cast<const char*>(a.pages + (l < RPT ? w.g : a.Hkv + w.g) * a.hd);
+        const u32x4 x = *reinterpret_cast<const u32x4*>(base + (((int64_t)page << a.t.sh) + (j & ((1 << a.t.sh) - 1))) * a.ldkv * 2 + lane_off);
+        if (l < RPT) k[i] = x;
+        else v[i] = x;
+    }
+    __device__ __forceinline__ bool full(const PagedTile& w, int step, unsigned ok) const { return ok == (1u << NG) - 1 && ((int64_t)step + 1) * NG * 16 <= w.len; }
+    __device__ __forceinline__ void blank(const PagedTile& w, int step, unsigned ok, int srow, int wave) {
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
-            const int row = i * PASS + wave * C::RPW, j = step * NG * 16 + row;
-            int page = id[(i * PASS) >> 4];
-            if (PASS > 16)
-#pragma unroll
-                for (int x = 1; x < PASS / 16; ++x) page = (wave * C::RPW) >> 4 == x ? id[((i * PASS) >> 4) + x] : page;
-            const bf16* p = base + (((int64_t)page << a.t.sh) + (j & ((1 << a.t.sh) - 1))) * a.ldkv + lane_off;
-            if (all) {
-                k[i] = *reinterpret_cast<const u32x4*>(p);
-                v[i] = *reinterpret_cast<const u32x4*>(p + vo);
-            } else {
-                k[i] = u32x4{0, 0, 0, 0};
-                v[i] = u32x4{0, 0, 0, 0};
-                if ((unsigned)page < (unsigned)a.t.n_pages && j + srow < w.len) {
-                    k[i] = *reinterpret_cast<const u32x4*>(p);
-                    v[i] = *reinterpret_cast<const u32x4*>(p + vo);
-                }
-            }
+            const int row = i * PASS + wave * C::RPW;
+            const bool there = ((ok >> (row >> 4)) & 1) && (int64_t)step * NG * 16 + row + srow < w.len;
+            k[i] = there ? k[i] : u32x4{0, 0, 0, 0};
+            v[i] = there ? v[i] : u32x4{0, 0, 0, 0};
         }
     }
     __device__ __forceinline__ bool clean() {
@@ -302,121 +354,220 @@ struct PStage {
         for (int i = 0; i < RPT; ++i) bad |= paged_clean(v[i]);
         return bad;
     }
-    __device__ __forceinline__ void park(char* kb, char* vb, int srow, int sch, int wave) const {
-#pragma unroll
-        for (int i = 0; i < RPT; ++i) {
-            const int row = i * PASS + wave * C::RPW + srow;
-            if (C::CPR * 8 == HDP || sch * 8 < HDP) {
-                *reinterpret_cast<u32x4*>(kb + row * C::PK + sch * 16) = k[i];
-                *reinterpret_cast<u32x4*>(vb + row * C::PV + sch * 16) = v[i];
-            }
+    // kp, vp: the lane's place (its row and chunk of the first load) in the K and V rows of the buffer
+    __device__ __forceinline__ void park(char* kp, char* vp, int l, int sch) const {
+        const int i = l % RPT;
+        if (C::CPR * 8 == HDP || sch * 8 < HDP) {
+            if (l < RPT) *reinterpret_cast<u32x4*>(kp + i * PASS * C::PK) = k[i];
+            else *reinterpret_cast<u32x4*>(vp + i * PASS * C::PV) = v[i];
         }
     }
 };
 
 // ---------------------------------------------------------------------------------------------------------------------------------
-// rows split over the waves
+// rows split over the waves.  The work of a launch is the 64-key steps of all (kv head, row tile) items in order; every worker (block) takes an equal, contiguous share of them, so
+// that no CU waits for another whatever the lengths are: 528 equal items on 512 block slots would take two rounds, the second nearly empty.  A worker walks from where its share begins
+// inside one item to where it ends inside another; an item that lies in one share is stored at once, of the others every worker leaves a part (at most two per worker) to the join.
 // ---------------------------------------------------------------------------------------------------------------------------------
+constexpr int MIN_SHARE = 8;       // steps: a shorter share would pay more for its parts than it gains
+
+// key steps of row tile t (0: no rows; a tile that sees no key takes one, fully masked, step)
+template <int R>
+__device__ __forceinline__ int tile_steps(const PagedAttn& a, int row0, int n, int len) {
+    const int rows = n * a.G;
+    if (row0 >= rows) return 0;
+    const int seen = min(paged_seen(a, len, n, (min(row0 + R, rows) - 1) / a.G), len);
+    return max((seen + 63) >> 6, 1);
+}
+
 template <int HDP, int QG, int NW>
 __global__ __launch_bounds__(NW * 64, QG == 2 || HDP > 128 ? 1 : 2) void attn_paged_tile_k(PagedAttn a) {
     using C = PCfg<HDP>;
-    constexpr int R = 32 * QG * NW, STAGE = 64 * (C::PK + C::PV);
+    constexpr int R = 32 * QG * NW, NT = NW * 64, STAGE = 64 * (C::PK + C::PV);
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ int dirty;
+    __shared__ int64_t scan[NW + 2];                       // wave sums | the first item's tile and its first step
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    PagedTile w;
-    int part;
-    {
-        // ids that differ by 8 run on one XCD: give every XCD a contiguous run of (kv head, part, tile) so that the tiles of one kv head share an L2; last rows (most keys) first
-        const int total = a.tiles * a.Hkv * a.nsplit, per = (total + 7) >> 3, id = blockIdx.x, i = (id & 7) * per + (id >> 3);
-        if ((id >> 3) >= per || i >= total) return;
-        const int tile = a.tiles - 1 - i % a.tiles, rest = i / a.tiles;
-        part = rest % a.nsplit;
-        w.g = rest / a.nsplit;
-        if (!paged_tile<R>(a, tile, w)) return;
-    }
-    const int per = paged_part<64>(w.len, a.nsplit);                                  // 64-key steps of a part
-    const int last_tok = (min(w.row0 + R, w.rows) - 1) / a.G;
-    const int kmax = paged_seen(a, w.len, w.n, last_tok);                              // keys that some row of the tile sees
-    const int t0 = part * per, t1 = min(t0 + per, (kmax + 63) >> 6);
-    const bool whole = per * 64 >= w.len;                                              // one part: the block writes the result itself
-    if (t0 >= t1 && !(whole && part == 0)) return;
-    const int row0 = w.row0 + wave * 32 * QG;
-    bf16x8 qf[QG][C::KS];
-    int seen[QG];
-    paged_load_q<HDP, QG>(a, w, row0, qf, seen);
-    const int seen_min = paged_seen(a, w.len, w.n, min(row0, w.rows - 1) / a.G);
-    const int diag = a.causal && w.n > 1 ? w.len - w.n : 0x7fffffff;                   // keys from here on are seen by some rows only
-
-    const int srow = lane / C::CPR, sch = lane % C::CPR;
-    const int64_t lane_off = srow * a.ldkv + (sch * 8 < a.hd ? sch * 8 : 0);
-    if (tid == 0) dirty = 0;
-    PStage<HDP, 4, NW> sg;
-    PState<HDP, QG> st;
-    st.clear();
-    unsigned groups = 0, next = 0;
-    if (t0 < t1) {
-        sg.ids(a, w, t0);
-        next = sg.valid(a);
-        sg.fetch(a, w, t0, next, lane_off, srow, wave);
-        sg.ids(a, w, t0 + 1);
-    }
-    __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-        char* kb = smem + ((t - t0) & 1) * STAGE;
-        if ((int64_t)(t + 1) * 64 > diag && __any(sg.clean()) && lane == 0) dirty = 1;
-        sg.park(kb, kb + 64 * C::PK, srow, sch, wave);
-        groups = next;
-        if (t + 1 < t1) {
-            next = sg.valid(a);
-            sg.fetch(a, w, t + 1, next, lane_off, srow, wave);
-            sg.ids(a, w, t + 2);
-        }
-        __syncthreads();                                                                // one barrier a step: the buffer written now was last read two steps ago
-        int vis[QG];
-#pragma unroll
-        for (int q = 0; q < QG; ++q) vis[q] = min(seen[q], w.len) - (t << 6);
-        paged_step<HDP, QG, 2>(kb, kb + 64 * C::PK, qf, st, a.sl2, (t << 6) + 64 > min(seen_min, w.len) || groups != 15u, vis, groups);
-    }
-    if (diag < w.len) {
-        __syncthreads();
-        if (dirty) paged_add_bad<HDP, QG>(a, w, max(diag, t0 << 6), min(t1 << 6, w.len), st, seen);
-    }
     const int h = lane >> 5, l31 = lane & 31;
+
+    // ---- the share.  Every block counts the steps of one kv head's tiles (thread: a run of m tiles) and finds where its share begins.
+    int64_t per_head, share, pos, end;
+    int worker, g, tile;
+    int64_t base;                                          // steps of the head's tiles before `tile`
+    {
+        const int m = (a.tiles + NT - 1) / NT, t0 = min(tid * m, a.tiles), t1 = min(t0 + m, a.tiles);
+        int s = 0;
+        for (int lo = 0, hi = a.t.S; lo < hi;) {           // the last slot whose numbers start at or before t0
+            const int mid = (lo + hi) >> 1;
+            if (paged_first_tile<R>(a, mid) <= t0) { s = mid; lo = mid + 1; } else hi = mid;
+        }
+        auto steps = [&](int t, int& s) {
+            while (s + 1 < a.t.S && paged_first_tile<R>(a, s + 1) <= t) ++s;
+            const int q0 = a.t.cu_q[s], n = a.t.cu_q[s + 1] - q0, first = paged_first_tile<R>(a, s);
+            if (t < first || q0 < 0 || n <= 0 || q0 + n > a.N) return 0;
+            return tile_steps<R>(a, (t - first) * R, n, paged_len(a.t, s));
+        };
+        int64_t mine = 0;
+        int s1 = s;
+        for (int t = t0; t < t1; ++t) mine += steps(t, s1);
+        int64_t x = mine;
 #pragma unroll
-    for (int q = 0; q < QG; ++q) {
-        const float l = st.l[q] + __shfl_xor(st.l[q], 32, 64);
-        const int r = row0 + 32 * q + l31;
-        if (r >= w.rows) continue;
-        const int tok = r / a.G, hq = w.g * a.G + (r - tok * a.G);
-        if (whole) {
-            const float inv = l > 0.f ? 1.f / l : l;                                   // l = 0: no key; NaN stays NaN
-            bf16* op = a.o + (int64_t)(w.q0 + tok) * a.ldo + hq * a.hd;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int64_t y = __shfl_up((long long)x, o, 64);
+            if (lane >= o) x += y;
+        }
+        if (lane == 63) scan[wave] = x;
+        if (tid == 0) scan[NW] = scan[NW + 1] = 0;
+        __syncthreads();
+        int64_t before = x - mine;
+        per_head = 0;
 #pragma unroll
-            for (int dt = 0; dt < C::DT; ++dt)
-#pragma unroll
-                for (int g4 = 0; g4 < 4; ++g4) {
-                    const int d = dt * 32 + g4 * 8 + h * 4;
-                    if (d < a.hd) {
-                        const bf16x4 ov = {(bf16)(st.o[q][dt][g4 * 4] * inv), (bf16)(st.o[q][dt][g4 * 4 + 1] * inv), (bf16)(st.o[q][dt][g4 * 4 + 2] * inv), (bf16)(st.o[q][dt][g4 * 4 + 3] * inv)};
-                        *reinterpret_cast<bf16x4*>(op + d) = ov;
-                    }
-                }
-        } else {
-            const int64_t rid = (int64_t)part * a.N * a.Hq + (int64_t)(w.q0 + tok) * a.Hq + hq;
-            float* op = a.part + rid * a.hd;
-#pragma unroll
-            for (int dt = 0; dt < C::DT; ++dt)
-#pragma unroll
-                for (int g4 = 0; g4 < 4; ++g4) {
-                    const int d = dt * 32 + g4 * 8 + h * 4;
-                    if (d < a.hd) *reinterpret_cast<f32x4*>(op + d) = f32x4{st.o[q][dt][g4 * 4], st.o[q][dt][g4 * 4 + 1], st.o[q][dt][g4 * 4 + 2], st.o[q][dt][g4 * 4 + 3]};
-                }
-            if (h == 0) {
-                float* ml = a.part + (int64_t)a.nsplit * a.N * a.Hq * a.hd + 2 * rid;
-                ml[0] = st.m[q];
-                ml[1] = l;
+        for (int i = 0; i < NW; ++i) {
+            before += i < wave ? scan[i] : 0;
+            per_head += scan[i];
+        }
+        const int64_t total = per_head * a.Hkv;
+        int64_t workers = total / MIN_SHARE;
+        workers = workers < 1 ? 1 : (workers > gridDim.x ? gridDim.x : workers);
+        share = (total + workers - 1) / workers;
+        // ids that differ by 8 run on one XCD: every XCD gets a contiguous run of shares, whose items share a kv head's keys in its L2
+        const int per = (int)((workers + 7) >> 3), id = blockIdx.x;
+        worker = (id & 7) * per + (id >> 3);
+        if ((id >> 3) >= per || worker >= workers || worker * share >= total) return;
+        pos = worker * share;
+        end = min(pos + share, total);
+        g = (int)(pos / per_head);
+        const int64_t off = pos - g * per_head;
+        if (off >= before && off < before + mine) {
+            int64_t at = before;
+            for (int t = t0; t < t1; ++t) {
+                const int c = steps(t, s);
+                if (off < at + c) { scan[NW] = t; scan[NW + 1] = at; break; }
+                at += c;
             }
+        }
+        __syncthreads();
+        tile = __builtin_amdgcn_readfirstlane((int)scan[NW]);
+        base = scan[NW + 1];
+        if (worker == 0 && tid == 0) reinterpret_cast<PShare*>(a.part)->steps = share;
+    }
+    const int64_t begin = pos;
+    const int srow = lane / C::CPR, sch = lane % C::CPR;
+    const unsigned lane_off = (unsigned)(srow * (int)a.ldkv + (sch * 8 < a.hd ? sch * 8 : 0)) * 2;
+    const int kp0 = (wave * C::RPW + srow) * C::PK + sch * 16, vp0 = 64 * C::PK + (wave * C::RPW + srow) * C::PV + sch * 16;
+    PItem* items = reinterpret_cast<PItem*>(reinterpret_cast<char*>(a.part) + 16);
+
+    while (pos < end && g < a.Hkv) {
+        PagedTile w;
+        w.g = g;
+        const int cost = paged_tile<R>(a, tile, w) ? tile_steps<R>(a, w.row0, w.n, w.len) : 0;
+        if (cost == 0) {                                   // a number without rows
+            if (++tile >= a.tiles) { tile = 0; base = 0; ++g; }
+            continue;
+        }
+        const int64_t start = g * per_head + base;
+        const int t0 = (int)(pos - start), t1 = (int)min((int64_t)cost, end - start);
+        const bool whole = t0 == 0 && t1 == cost;
+        if (t0 == 0 && tid == 0) items[(int64_t)g * a.tiles + tile] = PItem{start, cost};
+
+        const int row0 = w.row0 + wave * 32 * QG;
+        bf16x8 qf[QG][C::KS];
+        int seen[QG];
+        paged_load_q<HDP, QG>(a, w, row0, qf, seen);
+        const int seen_min = min(paged_seen(a, w.len, w.n, min(row0, w.rows - 1) / a.G), w.len);
+        const int diag = a.causal && w.n > 1 ? w.len - w.n : 0x7fffffff;              // keys from here on are seen by some rows only
+        using Stage = PStage<HDP, 4, NW>;
+        constexpr int NL = 2 * Stage::RPT;                                             // loads, and LDS writes, of a step
+        Stage sg;
+        PState<HDP, QG> st;
+        st.clear();
+        bool bad = false;
+        // zeros where there is no key; V elements that must not meet a zero of P set aside
+        auto tidy = [&](int t, unsigned ok) {
+            if (!sg.full(w, t, ok)) sg.blank(w, t, ok, srow, wave);
+            if ((int64_t)(t + 1) * 64 > diag) bad |= __any(sg.clean());
+        };
+        sg.load_ids(a, w, t0);
+        unsigned groups = sg.take_ids(a, w, t0);
+#pragma unroll
+        for (int l = 0; l < NL; ++l) sg.fetch(a, w, t0, l, lane_off, wave);
+        sg.load_ids(a, w, t0 + 1);
+        tidy(t0, groups);
+        __syncthreads();                                                                // the item before is done with the buffers
+        if (tid == 0) dirty = 0;
+        {
+            char* kb = smem + (t0 & 1) * STAGE;
+#pragma unroll
+            for (int l = 0; l < NL; ++l) sg.park(kb + kp0, kb + vp0, l, sch);
+        }
+        __syncthreads();
+        for (int t = t0; t < t1; ++t) {
+            const char* kb = smem + (t & 1) * STAGE;
+            char* kn = smem + ((t & 1) ^ 1) * STAGE;                                     // last read in the step before, which every wave has left
+            int vis[QG];
+#pragma unroll
+            for (int q = 0; q < QG; ++q) vis[q] = min(seen[q], w.len) - (t << 6);
+            const bool hide = (t << 6) + 64 > seen_min || groups != 15u;
+            if (t + 1 < t1) {
+                const unsigned next = sg.take_ids(a, w, t + 1);
+                paged_step<HDP, QG, 2>(kb, kb + 64 * C::PK, qf, st, a.sl2, hide, vis, groups,
+                    [&](int i, int n) {
+#pragma unroll
+                        for (int l = i * NL / n; l < (i + 1) * NL / n; ++l) sg.fetch(a, w, t + 1, l, lane_off, wave);
+                        if (i == n - 1) sg.load_ids(a, w, t + 2);
+                    },
+                    [&]() { tidy(t + 1, next); },
+                    [&](int i, int n) {
+#pragma unroll
+                        for (int l = i * NL / n; l < (i + 1) * NL / n; ++l) sg.park(kn + kp0, kn + vp0, l, sch);
+                    });
+                groups = next;
+            } else {
+                paged_step<HDP, QG, 2>(kb, kb + 64 * C::PK, qf, st, a.sl2, hide, vis, groups, [](int, int) {}, []() {}, [](int, int) {});
+            }
+            __syncthreads();
+        }
+        if (bad && lane == 0) dirty = 1;
+        if ((int64_t)t1 * 64 > diag) {
+            __syncthreads();
+            if (dirty) paged_add_bad<HDP, QG>(a, w, max(diag, t0 << 6), min(t1 << 6, w.len), st, seen);
+        }
+        float* part = tile_part<R>(a, worker, start <= begin ? 0 : 1);                 // the item that the share begins in, the item that it ends in
+#pragma unroll
+        for (int q = 0; q < QG; ++q) {
+            const float l = st.l[q] + __shfl_xor(st.l[q], 32, 64);
+            const int r = row0 + 32 * q + l31;
+            if (r >= w.rows) continue;
+            const int tok = r / a.G, hq = w.g * a.G + (r - tok * a.G);
+            if (whole) {
+                const float inv = l > 0.f ? 1.f / l : l;                               // l = 0: no key; NaN stays NaN
+                bf16* op = a.o + (int64_t)(w.q0 + tok) * a.ldo + hq * a.hd;
+#pragma unroll
+                for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+                    for (int g4 = 0; g4 < 4; ++g4) {
+                        const int d = dt * 32 + g4 * 8 + h * 4;
+                        if (d < a.hd) {
+                            const bf16x4 ov = {(bf16)(st.o[q][dt][g4 * 4] * inv), (bf16)(st.o[q][dt][g4 * 4 + 1] * inv), (bf16)(st.o[q][dt][g4 * 4 + 2] * inv), (bf16)(st.o[q][dt][g4 * 4 + 3] * inv)};
+                            *reinterpret_cast<bf16x4*>(op + d) = ov;
+                        }
+                    }
+            } else {
+                float* op = part + (int64_t)(r - w.row0) * a.hd;
+#pragma unroll
+                for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+                    for (int g4 = 0; g4 < 4; ++g4) {
+                        const int d = dt * 32 + g4 * 8 + h * 4;
+                        if (d < a.hd) *reinterpret_cast<f32x4*>(op + d) = f32x4{st.o[q][dt][g4 * 4], st.o[q][dt][g4 * 4 + 1], st.o[q][dt][g4 * 4 + 2], st.o[q][dt][g4 * 4 + 3]};
+                    }
+                if (h == 0) *reinterpret_cast<f32x2*>(part + R * a.hd + 2 * (r - w.row0)) = f32x2{st.m[q], l};
+            }
+        }
+        pos = start + t1;
+        if (t1 == cost) {
+            base += cost;
+            if (++tile >= a.tiles || base >= per_head) { tile = 0; base = 0; ++g; }
         }
     }
 }
@@ -446,35 +597,38 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_paged_keys_k(PagedAttn a) {
     char* vb = kb + 32 * C::PK;
     const int srow = lane / C::CPR, sch = lane % C::CPR;
     const int diag = a.causal && w.n > 1 ? w.len - w.n : 0x7fffffff;
-    const int64_t lane_off = srow * a.ldkv + (sch * 8 < a.hd ? sch * 8 : 0);
-    PStage<HDP, 2, 1> sg;
+    const unsigned lane_off = (unsigned)(srow * (int)a.ldkv + (sch * 8 < a.hd ? sch * 8 : 0)) * 2;
+    using Stage = PStage<HDP, 2, 1>;
+    Stage sg;
     unsigned next = 0;
+    auto fetch = [&](int t) {
+        next = sg.take_ids(a, w, t);
+#pragma unroll
+        for (int l = 0; l < 2 * Stage::RPT; ++l) sg.fetch(a, w, t, l, lane_off, 0);
+        sg.load_ids(a, w, t + NW);
+    };
     if (t0 + wave < t1) {
-        sg.ids(a, w, t0 + wave);
-        next = sg.valid(a);
-        sg.fetch(a, w, t0 + wave, next, lane_off, srow, 0);
-        sg.ids(a, w, t0 + wave + NW);
+        sg.load_ids(a, w, t0 + wave);
+        fetch(t0 + wave);
     }
     PState<HDP, 1> st;
     st.clear();
     bf16x8 qf[1][C::KS];
     int seen[1];
     paged_load_q<HDP, 1>(a, w, w.row0, qf, seen);
-    const int seen_min = paged_seen(a, w.len, w.n, w.row0 / a.G);
+    const int seen_min = min(paged_seen(a, w.len, w.n, w.row0 / a.G), w.len);
     bool dirty = false;
     for (int t = t0 + wave; t < t1; t += NW) {
+        if (!sg.full(w, t, next)) sg.blank(w, t, next, srow, 0);
         if ((int64_t)(t + 1) * 32 > diag) dirty |= __any(sg.clean());
-        sg.park(kb, vb, srow, sch, 0);
+#pragma unroll
+        for (int l = 0; l < 2 * Stage::RPT; ++l) sg.park(kb + srow * C::PK + sch * 16, vb + srow * C::PV + sch * 16, l, sch);
         const unsigned groups = next;
-        if (t + NW < t1) {
-            next = sg.valid(a);
-            sg.fetch(a, w, t + NW, next, lane_off, srow, 0);
-            sg.ids(a, w, t + 2 * NW);
-        }
+        if (t + NW < t1) fetch(t + NW);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");                          // the staged rows are read by other lanes of this wave
         __builtin_amdgcn_wave_barrier();
         int vis[1] = {min(seen[0], w.len) - (t << 5)};
-        paged_step<HDP, 1, 1>(kb, vb, qf, st, a.sl2, (t << 5) + 32 > min(seen_min, w.len) || groups != 3u, vis, groups);
+        paged_step<HDP, 1, 1>(kb, vb, qf, st, a.sl2, (t << 5) + 32 > seen_min || groups != 3u, vis, groups, [](int, int) {}, []() {}, [](int, int) {});
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
@@ -520,51 +674,84 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_paged_keys_k(PagedAttn a) {
     }
 }
 
-// The parts of one (row, q head), in a fixed order.  WPR waves work on it: lanes over quads of dims and over parts (64 / ql parts at once in a wave), so that even 64 parts are two rounds
-// of loads; the partial sums meet in LDS.  WPR = 4 from 9 parts on, else one wave, four of them to a block.
-template <int UNIT, int WPR>
-__global__ __launch_bounds__(256) void attn_paged_join_k(PagedAttn a, int ql) {
-    __shared__ float red[4][64 * 4];
+// Where the parts of one (row, q head) are: part p has its O at o(p) and its (max, sum) at ml(p)
+struct KeyParts {           // of attn_paged_keys_k
+    const float *o0, *ml0;
+    int64_t so, sml;
+    int parts;
+    template <int UNIT>
+    __device__ __forceinline__ bool find(const PagedAttn& a, int n, int hq, int s, int q0, int q1) {
+        const int len = paged_len(a.t, s), keys = paged_part<UNIT>(len, a.nsplit) * UNIT;
+        if (keys >= len) return false;                                                 // one part: written already
+        parts = (min(paged_seen(a, len, q1 - q0, n - q0), len) + keys - 1) / keys;
+        const int64_t stride = (int64_t)a.N * a.Hq, rid = (int64_t)n * a.Hq + hq;
+        o0 = a.part + rid * a.hd;
+        ml0 = a.part + a.nsplit * stride * a.hd + 2 * rid;
+        so = stride * a.hd;
+        sml = 2 * stride;
+        return true;
+    }
+    __device__ __forceinline__ const float* o(int p) const { return o0 + p * so; }
+    __device__ __forceinline__ const float* ml(int p) const { return ml0 + p * sml; }
+};
+
+template <int R>
+struct TileParts {          // of attn_paged_tile_k: the workers whose shares the item touches
+    const PagedAttn* a;
+    int64_t share, start, w0;
+    int row, parts;
+    __device__ __forceinline__ bool find(const PagedAttn& aa, int item) {
+        a = &aa;
+        share = max(reinterpret_cast<const PShare*>(aa.part)->steps, (int64_t)1);
+        const PItem it = reinterpret_cast<const PItem*>(reinterpret_cast<const char*>(aa.part) + 16)[item];
+        start = it.start;
+        w0 = start / share;
+        parts = (int)((start + it.cost - 1) / share - w0) + 1;
+        return parts > 1 && w0 >= 0 && w0 + parts <= aa.nsplit;
+    }
+    __device__ __forceinline__ const float* base(int p) const { return tile_part<R>(*a, w0 + p, start <= (w0 + p) * share ? 0 : 1); }
+    __device__ __forceinline__ const float* o(int p) const { return base(p) + (int64_t)row * a->hd; }
+    __device__ __forceinline__ const float* ml(int p) const { return base(p) + R * a->hd + 2 * row; }
+};
+
+// The parts of one (row, q head), added in a fixed order with weights 2^(m_p - m) by WPR waves: lanes over quads of dims and over parts (64 / ql parts at once in a wave; ql: lanes per
+// part, the power of two from hd / 4 on), so that even 64 parts are two rounds of loads for four waves.  red: 4 x 64 quads of LDS, used where WPR = 4 waves meet.
+template <int WPR, class Parts>
+__device__ __forceinline__ void paged_join_row(const PagedAttn& a, const Parts& ps, int ql, bf16* out, float (*red)[256]) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t id = WPR == 4 ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
-    if (id >= (int64_t)a.N * a.Hq) return;
-    const int n = __builtin_amdgcn_readfirstlane((int)(id / a.Hq)), hq = __builtin_amdgcn_readfirstlane((int)(id % a.Hq));
-    const int s = paged_slot_of_row(a.t.cu_q, a.t.S, n);
-    if (s >= a.t.S) return;
-    const int q0 = a.t.cu_q[s], q1 = a.t.cu_q[s + 1];
-    if (n < q0 || n >= q1 || q0 < 0 || q1 > a.N) return;
-    const int len = paged_len(a.t, s), keys = paged_part<UNIT>(len, a.nsplit) * UNIT;
-    if (keys >= len) return;                                                           // one part: written already
-    const int parts = (min(paged_seen(a, len, q1 - q0, n - q0), len) + keys - 1) / keys;      // <= 64
-    const int64_t stride = (int64_t)a.N * a.Hq, rid = (int64_t)n * a.Hq + hq;
-    float mp = -INFINITY, lp = 0.f;
-    if (lane < parts) {
-        const f32x2 v = *reinterpret_cast<const f32x2*>(a.part + a.nsplit * stride * a.hd + 2 * (lane * stride + rid));
-        mp = v[0];
-        lp = v[1];
-    }
-    const float m = wave_max(mp);
-    const float f = mp == -INFINITY ? (lp == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(mp - m);      // (a part of nothing but NaN has no maximum: its NaN stays)
-    const float sum = wave_sum(f * lp), inv = sum > 0.f ? 1.f / sum : sum;
-    const int quad = lane & (ql - 1), sub = lane / ql, np = 64 / ql;                   // ql: lanes per part, the power of two from hd / 4 on
+    float m = -INFINITY;
+    for (int c = 0; c < ps.parts; c += 64) m = fmaxf(m, c + lane < ps.parts ? ps.ml(c + lane)[0] : -INFINITY);
+    m = wave_max(m);
+    const int quad = lane & (ql - 1), sub = lane / ql, np = 64 / ql;
     const bool mine = quad * 4 < a.hd;
-    const float* x = a.part + rid * a.hd + quad * 4;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int p0 = (WPR == 4 ? wave * np : 0); p0 < parts; p0 += 4 * WPR * np) {
-        f32x4 v[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int p = p0 + k * WPR * np + sub;
-            v[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (mine && p < parts) v[k] = *reinterpret_cast<const f32x4*>(x + p * stride * a.hd);
+    float sum = 0.f;
+    for (int c = 0; c < ps.parts; c += 64) {
+        const int cn = min(ps.parts - c, 64);
+        float f = 0.f;
+        if (lane < cn) {
+            const f32x2 v = *reinterpret_cast<const f32x2*>(ps.ml(c + lane));
+            f = v[0] == -INFINITY ? (v[1] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(v[0] - m);      // (a part of nothing but NaN has no maximum: its NaN stays)
+            sum += f * v[1];
         }
+        for (int p0 = (WPR == 4 ? wave * np : 0); p0 < cn; p0 += 4 * WPR * np) {
+            f32x4 v[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int p = p0 + k * WPR * np + sub;
-            const float fp = __shfl(f, p < parts ? p : 0, 64);
-            if (p < parts) o += fp * v[k];
+            for (int k = 0; k < 4; ++k) {
+                const int p = p0 + k * WPR * np + sub;
+                v[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (mine && p < cn) v[k] = *reinterpret_cast<const f32x4*>(ps.o(c + p) + quad * 4);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int p = p0 + k * WPR * np + sub;
+                const float fp = __shfl(f, p < cn ? p : 0, 64);
+                if (p < cn) o += fp * v[k];
+            }
         }
     }
+    sum = wave_sum(sum);
+    const float inv = sum > 0.f ? 1.f / sum : sum;
     for (int d = ql; d < 64; d <<= 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], d, 64);
@@ -575,65 +762,92 @@ __global__ __launch_bounds__(256) void attn_paged_join_k(PagedAttn a, int ql) {
 #pragma unroll
         for (int k = 1; k < 4; ++k) o += *reinterpret_cast<const f32x4*>(&red[k][lane * 4]);
     }
-    if (sub == 0 && mine) *reinterpret_cast<bf16x4*>(a.o + (int64_t)n * a.ldo + hq * a.hd + quad * 4) = bf16x4{(bf16)(o[0] * inv), (bf16)(o[1] * inv), (bf16)(o[2] * inv), (bf16)(o[3] * inv)};
+    if (sub == 0 && mine) *reinterpret_cast<bf16x4*>(out + quad * 4) = bf16x4{(bf16)(o[0] * inv), (bf16)(o[1] * inv), (bf16)(o[2] * inv), (bf16)(o[3] * inv)};
+}
+
+// after attn_paged_keys_k: WPR = 4: a block for one (row, q head) (few rows, many parts); WPR = 1: four to a block
+template <int UNIT, int WPR>
+__global__ __launch_bounds__(256) void attn_paged_join_keys_k(PagedAttn a, int ql) {
+    __shared__ float red[4][256];
+    const int64_t id = WPR == 4 ? blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (id >= (int64_t)a.N * a.Hq) return;
+    const int n = __builtin_amdgcn_readfirstlane((int)(id / a.Hq)), hq = __builtin_amdgcn_readfirstlane((int)(id % a.Hq));
+    const int s = paged_slot_of_row(a.t.cu_q, a.t.S, n);
+    if (s >= a.t.S) return;
+    const int q0 = a.t.cu_q[s], q1 = a.t.cu_q[s + 1];
+    if (n < q0 || n >= q1 || q0 < 0 || q1 > a.N) return;
+    KeyParts ps;
+    if (ps.find<UNIT>(a, n, hq, s, q0, q1)) paged_join_row<WPR>(a, ps, ql, a.o + (int64_t)n * a.ldo + hq * a.hd, red);
+}
+
+// after attn_paged_tile_k: block = (item, every gridDim.y-th group of four rows), a wave for a row; items that no share boundary cuts leave at once
+template <int R>
+__global__ __launch_bounds__(256) void attn_paged_join_tiles_k(PagedAttn a, int ql) {
+    PagedTile w;
+    w.g = blockIdx.x / a.tiles;
+    if (!paged_tile<R>(a, blockIdx.x % a.tiles, w)) return;
+    TileParts<R> ps;
+    if (!ps.find(a, blockIdx.x)) return;
+    for (int r = blockIdx.y * 4 + (threadIdx.x >> 6); r < R && w.row0 + r < w.rows; r += gridDim.y * 4) {
+        const int tok = (w.row0 + r) / a.G, hq = w.g * a.G + w.row0 + r - tok * a.G;
+        ps.row = r;
+        paged_join_row<1>(a, ps, ql, a.o + (int64_t)(w.q0 + tok) * a.ldo + hq * a.hd, nullptr);
+    }
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
 struct Plan {
     bool keys;              // keys split over the waves (else rows)
-    int rows, unit, tiles, nsplit;
+    int rows, tiles;
+    int nsplit;             // keys kernel: parts
+    int workers;            // tile kernel: blocks
+    int64_t ws;             // bytes
 };
 
 // N, S: packed rows and slots; the lengths are on the device, the choice is made from the sizes alone.  A slot has N / S rows on average.
 Plan make_plan(int N, int S, int Hq, int Hkv, int hd, int max_keys) {
     const int G = Hq / Hkv;
     const int64_t rows = (int64_t)N * G;
-    Plan p;
+    Plan p = {};
     p.keys = rows <= 32 * (int64_t)S;
-    const int nw = hd > 128 ? 4 : 8;
     p.rows = p.keys ? 32 : 128;
-    p.unit = p.keys ? 32 * nw : 64;
     p.tiles = (int)(rows / p.rows) + S;
-    const int64_t full = rows / p.rows > S ? rows / p.rows : (N < S ? N : S);          // tiles that hold rows, about
-    const int64_t blocks = full * Hkv, want = p.keys ? 256 : 512;
-    const int64_t steps = ((int64_t)max_keys + p.unit - 1) / p.unit;
-    int64_t ns = blocks >= want ? 1 : (want + blocks - 1) / blocks;
-    if (ns > steps / 2) ns = steps / 2;
-    if (ns > 64) ns = 64;
-    p.nsplit = ns < 1 ? 1 : (int)ns;
+    p.nsplit = 1;
+    if (p.keys) {
+        const int unit = 32 * (hd > 128 ? 4 : 8);
+        const int64_t blocks = (int64_t)(N < S ? N : S) * Hkv, steps = ((int64_t)max_keys + unit - 1) / unit;
+        int64_t ns = (256 + blocks - 1) / blocks;
+        if (ns > steps / 2) ns = steps / 2;
+        if (ns > 64) ns = 64;
+        p.nsplit = ns < 1 ? 1 : (int)ns;
+        p.ws = p.nsplit > 1 ? 4 * (int64_t)p.nsplit * N * Hq * (hd + 2) : 0;
+    } else {
+        // two blocks of four waves fit a CU (one where head_dim is above 128)
+        const int64_t steps = (rows / p.rows + (S < N ? S : N)) * Hkv * (((int64_t)max_keys + 63) / 64), slots = hd > 128 ? 256 : 512;
+        p.workers = steps / MIN_SHARE >= slots ? (int)slots : (int)((steps / MIN_SHARE + 8) / 8 * 8);
+        p.ws = 16 + 16 * (int64_t)Hkv * p.tiles + 4 * (int64_t)p.workers * 2 * p.rows * (hd + 2);
+    }
     return p;
-}
-
-template <int UNIT>
-void join(const PagedAttn& a, hipStream_t st) {
-    int ql = 2;
-    while (ql * 4 < a.hd) ql <<= 1;
-    const int64_t rows = (int64_t)a.N * a.Hq;
-    if (a.nsplit > 8) hipLaunchKernelGGL((attn_paged_join_k<UNIT, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, ql);
-    else hipLaunchKernelGGL((attn_paged_join_k<UNIT, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, ql);
-}
-
-template <int HDP, int QG>
-void launch_tile(const PagedAttn& a, const Plan& p, hipStream_t st) {
-    using C = PCfg<HDP>;
-    constexpr int smem = 2 * 64 * (C::PK + C::PV);
-    UFV_ONCE_PER_DEVICE((void)hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_tile_k<HDP, QG, 4>), hipFuncAttributeMaxDynamicSharedMemorySize, smem););
-    const int64_t total = (int64_t)p.tiles * a.Hkv * p.nsplit;
-    hipLaunchKernelGGL((attn_paged_tile_k<HDP, QG, 4>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(256), smem, st, a);
-    if (p.nsplit > 1) join<64>(a, st);
 }
 
 template <int HDP>
 int launch(const PagedAttn& a, const Plan& p, hipStream_t st) {
     using C = PCfg<HDP>;
-    constexpr int NW = HDP > 128 ? 4 : 8;
+    int ql = 2;
+    while (ql * 4 < a.hd) ql <<= 1;
     if (p.keys) {
-        constexpr int smem = NW * 32 * (C::PK + C::PV);
+        constexpr int NW = HDP > 128 ? 4 : 8, smem = NW * 32 * (C::PK + C::PV);
         UFV_ONCE_PER_DEVICE((void)hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_keys_k<HDP, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, smem););
         hipLaunchKernelGGL((attn_paged_keys_k<HDP, NW>), dim3(p.tiles, p.nsplit, a.Hkv), dim3(NW * 64), smem, st, a);
-        if (p.nsplit > 1) join<32 * NW>(a, st);
+        const int64_t rows = (int64_t)a.N * a.Hq;
+        if (p.nsplit > 8) hipLaunchKernelGGL((attn_paged_join_keys_k<32 * NW, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, ql);
+        else if (p.nsplit > 1) hipLaunchKernelGGL((attn_paged_join_keys_k<32 * NW, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, ql);
     } else {
-        launch_tile<HDP, 1>(a, p, st);
+        constexpr int smem = 2 * 64 * (C::PK + C::PV);
+        UFV_ONCE_PER_DEVICE((void)hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_tile_k<HDP, 1, 4>), hipFuncAttributeMaxDynamicSharedMemorySize, smem););
+        hipLaunchKernelGGL((attn_paged_tile_k<HDP, 1, 4>), dim3(p.workers), dim3(256), smem, st, a);
+        const int items = p.tiles * a.Hkv;                                             // (a cut item's rows are spread over blocks where there are few items)
+        hipLaunchKernelGGL((attn_paged_join_tiles_k<128>), dim3(items, items >= 1024 ? 8 : 32), dim3(256), 0, st, a, ql);
     }
     UFV_CHECK_LAUNCH();
     return UFV_OK;
@@ -643,8 +857,7 @@ int launch(const PagedAttn& a, const Plan& p, hipStream_t st) {
 
 extern "C" int64_t ufv_attention_paged_ws_bytes(int N, int S, int Hq, int Hkv, int hd, int max_keys) {
     if (N <= 0 || S <= 0 || Hkv <= 0 || Hq < Hkv || hd <= 0) return 0;
-    const Plan p = make_plan(N, S, Hq, Hkv, hd, max_keys);
-    return p.nsplit > 1 ? 4 * (int64_t)p.nsplit * N * Hq * (hd + 2) : 0;
+    return make_plan(N, S, Hq, Hkv, hd, max_keys).ws;
 }
 
 extern "C" int ufv_attention_paged(const void* q, int64_t ldq, void* o, int64_t ldo, int N, int Hq, int Hkv, int hd, const void* pages, int n_pages, int page, int64_t ldkv,
@@ -656,19 +869,19 @@ extern "C" int ufv_attention_paged(const void* q, int64_t ldq, void* o, int64_t 
     UFV_REQUIRE(scale > 0.f && scale < INFINITY, "ufv_attention_paged: the scale must be positive and finite (%g)", (double)scale);
     UFV_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)o % 16 == 0 && ldq % 8 == 0 && ldo % 8 == 0, "ufv_attention_paged: rows must be 16-byte aligned (pitches %lld, %lld)", (long long)ldq,
                 (long long)ldo);
-    UFV_REQUIRE(ldkv >= 2 * (int64_t)Hkv * hd && (N == 1 || (ldq >= (int64_t)Hq * hd && ldo >= (int64_t)Hq * hd)), "ufv_attention_paged: a row pitch is too small");
+    UFV_REQUIRE(ldkv >= 2 * (int64_t)Hkv * hd && ldkv < 1 << 24 && (N == 1 || (ldq >= (int64_t)Hq * hd && ldo >= (int64_t)Hq * hd)), "ufv_attention_paged: a row pitch is out of range");
     UFV_REQUIRE((int64_t)N * Hq < 0x7fffffff && S < 1 << 24, "ufv_attention_paged: too many rows or slots (N=%d S=%d)", N, S);
     const Plan p = make_plan(N, S, Hq, Hkv, hd, max_pages << paged_log2(page));
-    UFV_REQUIRE((int64_t)p.tiles * Hkv * p.nsplit < 0x7fffffff - 8 && Hkv < 65536, "ufv_attention_paged: too many row tiles (N=%d S=%d)", N, S);
-    UFV_REQUIRE(p.nsplit == 1 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= ufv_attention_paged_ws_bytes(N, S, Hq, Hkv, hd, max_pages << paged_log2(page))),
-                "ufv_attention_paged: a workspace of %lld bytes is needed (%lld given)", (long long)ufv_attention_paged_ws_bytes(N, S, Hq, Hkv, hd, max_pages << paged_log2(page)), (long long)ws_bytes);
+    UFV_REQUIRE((int64_t)p.tiles * Hkv < 0x7fffffff && Hkv < 65536, "ufv_attention_paged: too many row tiles (N=%d S=%d)", N, S);
+    UFV_REQUIRE(p.ws == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= p.ws), "ufv_attention_paged: a 16-byte aligned workspace of %lld bytes is needed (%lld given)", (long long)p.ws,
+                (long long)ws_bytes);
     PagedAttn a;
     a.q = (const bf16*)q; a.pages = (const bf16*)pages; a.o = (bf16*)o;
     a.ldq = ldq; a.ldo = ldo; a.ldkv = ldkv;
     a.t = PagedTable{block_table, ld_table, max_pages, cu_q, kv_len, S, n_pages, paged_log2(page)};
     a.N = N; a.Hq = Hq; a.Hkv = Hkv; a.G = Hq / Hkv; a.hd = hd; a.causal = causal != 0;
     a.sl2 = scale * 1.4426950408889634f;
-    a.nsplit = p.nsplit; a.tiles = p.tiles; a.part = (float*)ws;
+    a.nsplit = p.keys ? p.nsplit : p.workers; a.tiles = p.tiles; a.part = (float*)ws;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (hd <= 32) return launch<32>(a, p, st);
     if (hd <= 64) return launch<64>(a, p, st);
