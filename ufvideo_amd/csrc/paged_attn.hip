@@ -13,6 +13,10 @@
 // Either may be split further over the keys by blocks (few tiles on 256 CUs); the parts leave (max, sum, un-normalised O) in 32 bits in the workspace and attn_paged_join_k adds them in order.
 #include "paged.h"
 
+#ifndef BIGQ
+#define BIGQ 1
+#define BIGN 8
+#endif
 namespace {
 
 typedef __attribute__((ext_vector_type(2))) float f32x2;
@@ -94,13 +98,23 @@ __device__ __forceinline__ bf16x8 pack8(const float* p) {
     return r;
 }
 
+// K and V rows in LDS: P bytes a row, chunk c (16 bytes) of row r at slot c ^ f(r) -- without padding, so that a row can come straight from memory, and free of bank conflicts: eight rows'
+// same chunk (a K fragment) and four rows' neighbouring chunk pairs (a transposing V read) fall on different banks.  The matrix instructions' addresses are one per lane, XORed with constants.
 template <int HDP>
 struct PCfg {
     static constexpr int KS = HDP / 16, DT = HDP / 32;
-    static constexpr int CPR = HDP <= 32 ? 4 : (HDP <= 64 ? 8 : (HDP <= 128 ? 16 : 32));     // lanes that fetch one cache row, 16 bytes each (a power of two; HDP 96: four idle)
+    static constexpr int CPR = HDP <= 32 ? 4 : (HDP <= 64 ? 8 : (HDP <= 128 ? 16 : 32));     // chunks of a row, lanes that fetch it (a power of two; HDP 96: four more than it has)
     static constexpr int RPW = 64 / CPR;                                                     // rows of one wave load: at most 16, so all of one page
-    static constexpr int PK = HDP * 2 + 16;                                                  // K row pitch: an odd number of 16-byte slots, conflict-free b128 reads
-    static constexpr int PV = HDP == 32 ? 64 : (HDP <= 96 ? 192 : (HDP == 128 ? 320 : 576)); // V row pitch: 64 or 192 mod 256, conflict-free transposing reads
+    static constexpr int P = CPR * 16;
+    __device__ static __forceinline__ int f(int r) { return CPR >= 16 ? 2 * (r & 7) : (CPR == 8 ? r & 7 : (r >> 2) & 3); }
+    // lane (l31, h): K row l31 chunk 2 ks + h at kaddr ^ (ks << 5); 32 rows on: + 32 P
+    __device__ static __forceinline__ int kaddr(int lane) { return (lane & 31) * P + 16 * ((lane >> 5) ^ f(lane & 31)); }
+    // lane's part of the transposing reads of keys 4 h .. 4 h + 3 (the second: 8 keys on), dims 32 dt ..: vaddr ^ (dt << 6), second: (vaddr ^ VX) + 8 P; 16 keys on: + 16 P
+    static constexpr int VX = CPR == 4 ? 32 : 0;
+    __device__ static __forceinline__ int vaddr(int lane) {
+        const int r = 4 * (lane >> 5) + ((lane & 15) >> 2), u = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+        return r * P + 16 * (u ^ f(r)) + 8 * (lane & 1);
+    }
 };
 
 // One 32-key half tile in LDS against QG groups of 32 rows: S^T, running softmax, O^T.
@@ -122,15 +136,15 @@ struct PState {
     }
 };
 
-// at_qk(i) / at_pv(i, n) run behind the i-th product of S^T / behind the i-th of the n products of O^T: the loads and LDS writes of the next step go there, a few at a time -- issued in
-// one go they hold the wave for 1300 + 700 of the 4900 cycles of a step (the memory pipe takes one 1 KB load in 16 cycles), behind the products they cost nothing.
-template <int HDP, int QG, int NH, class FQ, class FB, class FP>
-__device__ __forceinline__ void paged_step(const char* kb, const char* vb, const bf16x8 (&qf)[QG][HDP / 16], PState<HDP, QG>& st, float sl2, bool hide, const int (&vis)[QG], unsigned groups,
-                                           FQ&& at_qk, FB&& before_pv, FP&& at_pv) {
+// at_qk(i, n, next) runs behind the i-th of the n products of S^T: the loads of the next step (memory -> LDS at `next`) go there, a few at a time -- issued in one go they hold the wave for
+// 1300 of the 4900 cycles of a step (the memory pipe takes one 1 KB load in 16 cycles), behind the products they cost little.  kb, vb, next do not overlap (__restrict__ lets the compiler
+// keep the loads in flight across the reads: who issues them waits for them before the barrier that publishes them).
+template <int HDP, int QG, int NH, class FQ>
+__device__ __forceinline__ void paged_step(const char* __restrict__ kb, const char* __restrict__ vb, char* __restrict__ next, const bf16x8 (&qf)[QG][HDP / 16], PState<HDP, QG>& st, float sl2, bool hide, const int (&vis)[QG], unsigned groups,
+                                           FQ&& at_qk) {
     using C = PCfg<HDP>;
-    const int lane = threadIdx.x & 63, h = lane >> 5, l31 = lane & 31;
-    const int k_off = l31 * C::PK + h * 16;
-    const int v_off = (4 * h + ((lane & 15) >> 2)) * C::PV + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    const int k_off = C::kaddr(lane), v_off = C::vaddr(lane);
     // Left to itself the compiler puts every LDS read right in front of the matrix instruction that needs it and waits out the LDS latency 32 times a step.  The order below is pinned
     // (sched_barrier): AHEAD fragments are in flight at any time, the V reads start before the exponentials, and the second half's exponentials go between the first half's products.
     constexpr int AHEAD = 4, NR = C::KS * NH, PRE = AHEAD < NR ? AHEAD : NR;
@@ -143,7 +157,7 @@ __device__ __forceinline__ void paged_step(const char* kb, const char* vb, const
             for (int r = 0; r < 16; ++r) s[q][hh][r] = 0.f;
     {
         bf16x8 kf[PRE];
-        auto read = [&](int i) { return *reinterpret_cast<const bf16x8*>(kb + (i % NH) * 32 * C::PK + k_off + (i / NH) * 32); };
+        auto read = [&](int i) { return *reinterpret_cast<const bf16x8*>(kb + (k_off ^ ((i / NH) << 5)) + (i % NH) * 32 * C::P); };
 #pragma unroll
         for (int i = 0; i < PRE; ++i) kf[i] = read(i);
         __builtin_amdgcn_sched_barrier(0);
@@ -152,7 +166,7 @@ __device__ __forceinline__ void paged_step(const char* kb, const char* vb, const
 #pragma unroll
             for (int q = 0; q < QG; ++q) s[q][i % NH] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i % PRE], qf[q][i / NH], s[q][i % NH], 0, 0, 0);
             if (i + PRE < NR) kf[i % PRE] = read(i + PRE);
-            at_qk(i, NR);
+            at_qk(i, NR, next);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -189,11 +203,10 @@ __device__ __forceinline__ void paged_step(const char* kb, const char* vb, const
         }
         msub[q] = st.m[q] == -INFINITY ? 0.f : st.m[q];
     }
-    before_pv();
     constexpr int NM = 2 * C::DT, NV = NM * NH, PREV = AHEAD < NV ? AHEAD : NV, EPM = (16 + NM - 1) / NM;      // products of a half, of the step; elements per product
     bf16x4 vf[PREV][2];
     auto readv = [&](int i, int u) {                       // product i: keys 16 (i / DT) .., dims 32 (i % DT) ..
-        const char* vp = vb + 16 * (i / C::DT) * C::PV + v_off + (i % C::DT) * 64 + u * 8 * C::PV;
+        const char* vp = vb + ((v_off ^ ((i % C::DT) << 6)) ^ (u ? C::VX : 0)) + (16 * (i / C::DT) + 8 * u) * C::P;
         return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((bf16x4 __attribute__((address_space(3)))*)(vp));
     };
 #pragma unroll
@@ -229,7 +242,6 @@ __device__ __forceinline__ void paged_step(const char* kb, const char* vb, const
 #pragma unroll
         for (int q = 0; q < QG; ++q) st.o[q][i % C::DT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, pf[q][(i % NM) / C::DT], st.o[q][i % C::DT], 0, 0, 0);
         if (i + PREV < NV) { vf[i % PREV][0] = readv(i + PREV, 0); vf[i % PREV][1] = readv(i + PREV, 1); }
-        at_pv(i, NV);
         if (NH == 2 && i < NM) exps(1, EPM * i < 16 ? EPM * i : 16, EPM * (i + 1) < 16 ? EPM * (i + 1) : 16);
         __builtin_amdgcn_sched_barrier(0);
     }
@@ -242,7 +254,8 @@ __device__ __forceinline__ void paged_step(const char* kb, const char* vb, const
 // p > 0 times Inf or NaN is Inf or NaN).
 template <int HDP, int QG>
 __device__ __forceinline__ void paged_add_bad(const PagedAttn& a, const PagedTile& w, int j0, int j1, PState<HDP, QG>& st, const int (&seen)[QG]) {
-    const int h = (threadIdx.x & 63) >> 5;
+    int h = (threadIdx.x & 63) >> 5;
+    asm volatile("" : "+v"(h));                           // opaque: nothing of this path is kept in registers outside it
     for (int j = j0; j < j1; ++j) {
         const int64_t at = paged_row(a.t, w.s, j);
         if (at < 0) continue;
@@ -280,7 +293,9 @@ __device__ __forceinline__ bool paged_clean(u32x4& v) {
 // The lane's rows of the tile as B operands (lane: row l31 of the group, dims 16 ks + 8 h ..), and what they see.  Rows behind the tile's last take the last one's q; they are not stored.
 template <int HDP, int QG>
 __device__ __forceinline__ void paged_load_q(const PagedAttn& a, const PagedTile& w, int row0, bf16x8 (&qf)[QG][HDP / 16], int (&seen)[QG]) {
-    const int lane = threadIdx.x & 63, h = lane >> 5, l31 = lane & 31;
+    const int lane = threadIdx.x & 63, l31 = lane & 31;
+    int h = lane >> 5;
+    asm volatile("" : "+v"(h));                           // opaque: the bounds of the chunks must not be kept in registers over the walk
 #pragma unroll
     for (int q = 0; q < QG; ++q) {
         const int r = min(row0 + 32 * q + l31, w.rows - 1), tok = r / a.G, hq = w.g * a.G + (r - tok * a.G);
@@ -294,73 +309,45 @@ __device__ __forceinline__ void paged_load_q(const PagedAttn& a, const PagedTile
     }
 }
 
-// Staging of NG groups of 16 keys by NWS waves, cache -> registers -> LDS.  A wave load covers RPW <= 16 rows that start at a multiple of RPW, and a page holds whole groups of 16
-// tokens: the page is the same for the whole load and its address a scalar; the lane's part of the address does not change.  Lanes whose chunk lies behind hd (padded head dims) fetch
-// chunk 0: their K meets zeros in Q, their V columns are not stored.  The ids come by a vector load (lane i: group i) behind the rows of the step before: a scalar load would share its
-// counter with the LDS reads and be waited out before the next barrier, every step.
+// Fetching NG groups of 16 keys (a step) by NWS waves.  A wave load covers RPW <= 16 rows that start at a multiple of RPW, and a page holds whole groups of 16 tokens: the page is the same
+// for the whole load and its address a scalar; the lane's part of the address does not change.  It is a buffer load whose base is the load's first row and whose range ends behind the last row
+// that is a key: what lies outside -- tokens behind the last one, a page outside the pool -- comes back as zeros and is not read.  Lanes whose chunk lies behind hd (padded head dims) fetch
+// chunk 0: their K meets zeros in Q, their V columns are not stored.  Page ids: one vector load holds those of 64 groups, one a lane.
 template <int HDP, int NG, int NWS>
-struct PStage {
+struct PFetch {
     using C = PCfg<HDP>;
-    static constexpr int PASS = NWS * C::RPW, RPT = 16 * NG / PASS;
+    static constexpr int PASS = NWS * C::RPW, RPT = 16 * NG / PASS, NL = 2 * RPT;       // rows of a pass, passes, loads of a wave (K, then V)
+    static constexpr int SPC = 64 / NG;                                                 // steps whose ids one load holds
     static_assert(RPT >= 1 && RPT * PASS == 16 * NG, "whole passes");
-    u32x4 k[RPT], v[RPT];
-    int idv;                // lane i < NG: page id of the next step's group i
-    int id[NG];             // the same as scalars, -1 where there is no key or no such page
+    int id[NG];             // page ids of a step, -1 where there is no key or no such page
 
-    __device__ __forceinline__ void load_ids(const PagedAttn& a, const PagedTile& w, int step) {
-        const int64_t j = ((int64_t)step * NG + (threadIdx.x & (NG - 1))) * 16;
-        const int i = min((int)(j >> a.t.sh), a.t.width - 1);
-        idv = a.t.table[(int64_t)w.s * a.t.ld + i];
+    // lane i: the id of group 64 c + i (tokens and groups stay below 2^31; past the table's last entry: that one)
+    __device__ __forceinline__ static int chunk(const PagedAttn& a, const PagedTile& w, int c) {
+        const int i = min((int)(((unsigned)c * 64u + (threadIdx.x & 63)) << 4 >> a.t.sh), a.t.width - 1);
+        return *reinterpret_cast<const int*>(reinterpret_cast<const char*>(a.t.table + (int64_t)w.s * a.t.ld) + (unsigned)i * 4u);
     }
-    // scalars of the ids loaded for `step`; bit i: group i has keys
-    __device__ __forceinline__ unsigned take_ids(const PagedAttn& a, const PagedTile& w, int step) {
+    // the ids of `step` out of its chunk; bit i: group i has keys.  From step `end` on there is nothing: no ids, nothing is read
+    __device__ __forceinline__ unsigned take(const PagedAttn& a, const PagedTile& w, int ids, int step, int end) {
         unsigned ok = 0;
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
-            id[i] = __builtin_amdgcn_readlane(idv, i);
-            const bool there = ((int64_t)step * NG + i) * 16 < w.len && (unsigned)id[i] < (unsigned)a.t.n_pages;
+            id[i] = __builtin_amdgcn_readlane(ids, (step % SPC) * NG + i);
+            const bool there = step < end && (step * NG + i) * 16 < w.len && (unsigned)id[i] < (unsigned)a.t.n_pages;
             id[i] = there ? id[i] : -1;
             ok |= there ? 1u << i : 0u;
         }
         return ok;
     }
-    // load l (of 2 RPT: K rows, then V rows) of the step whose ids were taken.  It is never conditional: where there is no page it reads page 0, behind the last token whatever the page
-    // holds; blank() puts zeros there before the rows are parked.  lane_off: byte offset of the lane's row and chunk inside a load; wave: the wave's place among the NWS
-    __device__ __forceinline__ void fetch(const PagedAttn& a, const PagedTile& w, int step, int l, unsigned lane_off, int wave) {
-        const int i = l % RPT, row = i * PASS + wave * C::RPW, j = step * NG * 16 + row;
+    // load l (l < RPT: K, else V) of the step whose ids were taken: its base, and the bytes of its range; wave: the wave's place among the NWS
+    __device__ __forceinline__ bf16* rows(const PagedAttn& a, const PagedTile& w, int step, int l, int wave, int& bytes) const {
+        const int i = l % RPT, j = step * NG * 16 + i * PASS + wave * C::RPW;
         int page = id[(i * PASS) >> 4];
         if (PASS > 16)
 #pragma unroll
             for (int x = 1; x < PASS / 16; ++x) page = (wave * C::RPW) >> 4 == x ? id[((i * PASS) >> 4) + x] : page;
-        page = max(page, 0);
-        const char* base = reinterpret_cast<const char*>(a.pages + (l < RPT ? w.g : a.Hkv + w.g) * a.hd);
-        const u32x4 x = *reinterpret_cast<const u32x4*>(base + (((int64_t)page << a.t.sh) + (j & ((1 << a.t.sh) - 1))) * a.ldkv * 2 + lane_off);
-        if (l < RPT) k[i] = x;
-        else v[i] = x;
-    }
-    __device__ __forceinline__ bool full(const PagedTile& w, int step, unsigned ok) const { return ok == (1u << NG) - 1 && ((int64_t)step + 1) * NG * 16 <= w.len; }
-    __device__ __forceinline__ void blank(const PagedTile& w, int step, unsigned ok, int srow, int wave) {
-#pragma unroll
-        for (int i = 0; i < RPT; ++i) {
-            const int row = i * PASS + wave * C::RPW;
-            const bool there = ((ok >> (row >> 4)) & 1) && (int64_t)step * NG * 16 + row + srow < w.len;
-            k[i] = there ? k[i] : u32x4{0, 0, 0, 0};
-            v[i] = there ? v[i] : u32x4{0, 0, 0, 0};
-        }
-    }
-    __device__ __forceinline__ bool clean() {
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < RPT; ++i) bad |= paged_clean(v[i]);
-        return bad;
-    }
-    // kp, vp: the lane's place (its row and chunk of the first load) in the K and V rows of the buffer
-    __device__ __forceinline__ void park(char* kp, char* vp, int l, int sch) const {
-        const int i = l % RPT;
-        if (C::CPR * 8 == HDP || sch * 8 < HDP) {
-            if (l < RPT) *reinterpret_cast<u32x4*>(kp + i * PASS * C::PK) = k[i];
-            else *reinterpret_cast<u32x4*>(vp + i * PASS * C::PV) = v[i];
-        }
+        const int keys = page < 0 ? 0 : min(max(w.len - j, 0), C::RPW);
+        bytes = keys > 0 ? keys * (int)a.ldkv * 2 - ((int)a.ldkv - a.hd) * 2 : 0;       // up to the end of the last key's chunks of this head
+        return const_cast<bf16*>(a.pages) + (((int64_t)max(page, 0) << a.t.sh) + (j & ((1 << a.t.sh) - 1))) * a.ldkv + (l < RPT ? w.g : a.Hkv + w.g) * a.hd;
     }
 };
 
@@ -380,10 +367,10 @@ __device__ __forceinline__ int tile_steps(const PagedAttn& a, int row0, int n, i
     return max((seen + 63) >> 6, 1);
 }
 
-template <int HDP, int QG, int NW>
+template <int HDP, int QG, int NW, int NS>
 __global__ __launch_bounds__(NW * 64, QG == 2 || HDP > 128 ? 1 : 2) void attn_paged_tile_k(PagedAttn a) {
     using C = PCfg<HDP>;
-    constexpr int R = 32 * QG * NW, NT = NW * 64, STAGE = 64 * (C::PK + C::PV);
+    constexpr int R = 32 * QG * NW, NT = NW * 64, HALF = 64 * C::P, STAGE = 2 * HALF;      // a step's K rows, its K and V rows
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ int dirty;
     __shared__ int64_t scan[NW + 2];                       // wave sums | the first item's tile and its first step
@@ -452,9 +439,8 @@ __global__ __launch_bounds__(NW * 64, QG == 2 || HDP > 128 ? 1 : 2) void attn_pa
         if (worker == 0 && tid == 0) reinterpret_cast<PShare*>(a.part)->steps = share;
     }
     const int64_t begin = pos;
-    const int srow = lane / C::CPR, sch = lane % C::CPR;
+    const int srow = lane / C::CPR, sch = (lane % C::CPR) ^ C::f(wave * C::RPW + srow);  // the lane's row in a load, the chunk that belongs into its place
     const unsigned lane_off = (unsigned)(srow * (int)a.ldkv + (sch * 8 < a.hd ? sch * 8 : 0)) * 2;
-    const int kp0 = (wave * C::RPW + srow) * C::PK + sch * 16, vp0 = 64 * C::PK + (wave * C::RPW + srow) * C::PV + sch * 16;
     PItem* items = reinterpret_cast<PItem*>(reinterpret_cast<char*>(a.part) + 16);
 
     while (pos < end && g < a.Hkv) {
@@ -476,62 +462,81 @@ __global__ __launch_bounds__(NW * 64, QG == 2 || HDP > 128 ? 1 : 2) void attn_pa
         paged_load_q<HDP, QG>(a, w, row0, qf, seen);
         const int seen_min = min(paged_seen(a, w.len, w.n, min(row0, w.rows - 1) / a.G), w.len);
         const int diag = a.causal && w.n > 1 ? w.len - w.n : 0x7fffffff;              // keys from here on are seen by some rows only
-        using Stage = PStage<HDP, 4, NW>;
-        constexpr int NL = 2 * Stage::RPT;                                             // loads, and LDS writes, of a step
-        Stage sg;
+        using F = PFetch<HDP, 4, NW>;
+        constexpr int NL = F::NL, D = NS - 1;                                          // steps ahead
+        F fe;
         PState<HDP, QG> st;
         st.clear();
         bool bad = false;
-        // zeros where there is no key; V elements that must not meet a zero of P set aside
-        auto tidy = [&](int t, unsigned ok) {
-            if (!sg.full(w, t, ok)) sg.blank(w, t, ok, srow, wave);
-            if ((int64_t)(t + 1) * 64 > diag) bad |= __any(sg.clean());
+        auto dma = [&](int t, int l, char* buf) {
+            int bytes;
+            bf16* base = fe.rows(a, w, t, l, wave, bytes);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc(base, 0, bytes, 0x20000), LDS_PTR(buf + (l < NL / 2 ? 0 : HALF) + ((l % (NL / 2)) * F::PASS + wave * C::RPW) * C::P), 16, lane_off, 0, 0, 0);
         };
-        sg.load_ids(a, w, t0);
-        unsigned groups = sg.take_ids(a, w, t0);
+        // waits until this wave's loads of step t have arrived, those of the steps behind it may still be under way (in order: at most NL of each); then takes care of elements that must
+        // not meet a zero of P.  The barrier behind it publishes the step.
+        auto arrived = [&](int t, char* buf) {
+            if (D > 2 && t + 2 < t1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NL < 63 ? 2 * NL : 63) : "memory");
+            else if (D > 1 && t + 1 < t1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL < 63 ? NL : 63) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (t * 64 + 64 > diag) {
 #pragma unroll
-        for (int l = 0; l < NL; ++l) sg.fetch(a, w, t0, l, lane_off, wave);
-        sg.load_ids(a, w, t0 + 1);
-        tidy(t0, groups);
+                for (int i = 0; i < NL / 2; ++i) {
+                    u32x4* p = reinterpret_cast<u32x4*>(buf + HALF + (i * F::PASS + wave * C::RPW) * C::P + lane * 16);
+                    u32x4 v = *p;
+                    if (paged_clean(v)) {
+                        bad = true;
+                        *p = v;
+                    }
+                }
+            }
+        };
+        int ids = F::chunk(a, w, t0 / F::SPC), ids2 = F::chunk(a, w, t0 / F::SPC + 1);    // of the step to be fetched next and its neighbours, of the chunk behind it
+        unsigned groups[NS];                                                            // which groups of 16 keys of the steps under way exist
         __syncthreads();                                                                // the item before is done with the buffers
         if (tid == 0) dirty = 0;
-        {
-            char* kb = smem + (t0 & 1) * STAGE;
 #pragma unroll
-            for (int l = 0; l < NL; ++l) sg.park(kb + kp0, kb + vp0, l, sch);
+        for (int d = 0; d < D; ++d) {
+            if (d > 0 && (t0 + d) % F::SPC == 0) { ids = ids2; ids2 = F::chunk(a, w, (t0 + d) / F::SPC + 1); }
+            groups[d] = fe.take(a, w, ids, t0 + d, t1);
+            if (t0 + d < t1)
+#pragma unroll
+                for (int l = 0; l < NL; ++l) dma(t0 + d, l, smem + d * STAGE);
         }
+        arrived(t0, smem);
         __syncthreads();
+        int cur = 0;                                                                    // the step's buffer in the ring
         for (int t = t0; t < t1; ++t) {
-            const char* kb = smem + (t & 1) * STAGE;
-            char* kn = smem + ((t & 1) ^ 1) * STAGE;                                     // last read in the step before, which every wave has left
+            const char* kb = smem + cur * STAGE;
+            char* kn = smem + (cur == 0 ? NS - 1 : cur - 1) * STAGE;                     // of step t - 1, which every wave has left: step t + D goes there
+            cur = cur == NS - 1 ? 0 : cur + 1;
             int vis[QG];
 #pragma unroll
             for (int q = 0; q < QG; ++q) vis[q] = min(seen[q], w.len) - (t << 6);
-            const bool hide = (t << 6) + 64 > seen_min || groups != 15u;
-            if (t + 1 < t1) {
-                const unsigned next = sg.take_ids(a, w, t + 1);
-                paged_step<HDP, QG, 2>(kb, kb + 64 * C::PK, qf, st, a.sl2, hide, vis, groups,
-                    [&](int i, int n) {
+            const unsigned keys = groups[0];
 #pragma unroll
-                        for (int l = i * NL / n; l < (i + 1) * NL / n; ++l) sg.fetch(a, w, t + 1, l, lane_off, wave);
-                        if (i == n - 1) sg.load_ids(a, w, t + 2);
-                    },
-                    [&]() { tidy(t + 1, next); },
-                    [&](int i, int n) {
+            for (int d = 0; d + 1 < D; ++d) groups[d] = groups[d + 1];
+            if ((t + D) % F::SPC == 0) { ids = ids2; ids2 = F::chunk(a, w, (t + D) / F::SPC + 1); }
+            groups[D - 1] = fe.take(a, w, ids, t + D, t1);
+            const bool more = t + D < t1;
+            paged_step<HDP, QG, 2>(kb, kb + HALF, kn, qf, st, a.sl2, (t << 6) + 64 > seen_min || keys != 15u, vis, keys, [&](int i, int n, char* next) {
+                if (more) {
 #pragma unroll
-                        for (int l = i * NL / n; l < (i + 1) * NL / n; ++l) sg.park(kn + kp0, kn + vp0, l, sch);
-                    });
-                groups = next;
-            } else {
-                paged_step<HDP, QG, 2>(kb, kb + 64 * C::PK, qf, st, a.sl2, hide, vis, groups, [](int, int) {}, []() {}, [](int, int) {});
-            }
+                    for (int l = i * NL / n; l < (i + 1) * NL / n; ++l) dma(t + D, l, next);
+                }
+            });
+            if (t + 1 < t1) arrived(t + 1, smem + cur * STAGE);
             __syncthreads();
         }
+        bad = __any(bad);
+        bad = __any(bad);
         if (bad && lane == 0) dirty = 1;
         if ((int64_t)t1 * 64 > diag) {
             __syncthreads();
             if (dirty) paged_add_bad<HDP, QG>(a, w, max(diag, t0 << 6), min(t1 << 6, w.len), st, seen);
         }
+        int he = h;                                                                     // opaque: what follows from it (dims, bounds, addresses) must not be kept in registers over the walk
+        asm volatile("" : "+v"(he));
         float* part = tile_part<R>(a, worker, start <= begin ? 0 : 1);                 // the item that the share begins in, the item that it ends in
 #pragma unroll
         for (int q = 0; q < QG; ++q) {
@@ -546,7 +551,7 @@ __global__ __launch_bounds__(NW * 64, QG == 2 || HDP > 128 ? 1 : 2) void attn_pa
                 for (int dt = 0; dt < C::DT; ++dt)
 #pragma unroll
                     for (int g4 = 0; g4 < 4; ++g4) {
-                        const int d = dt * 32 + g4 * 8 + h * 4;
+                        const int d = dt * 32 + g4 * 8 + he * 4;
                         if (d < a.hd) {
                             const bf16x4 ov = {(bf16)(st.o[q][dt][g4 * 4] * inv), (bf16)(st.o[q][dt][g4 * 4 + 1] * inv), (bf16)(st.o[q][dt][g4 * 4 + 2] * inv), (bf16)(st.o[q][dt][g4 * 4 + 3] * inv)};
                             *reinterpret_cast<bf16x4*>(op + d) = ov;
@@ -558,10 +563,10 @@ __global__ __launch_bounds__(NW * 64, QG == 2 || HDP > 128 ? 1 : 2) void attn_pa
                 for (int dt = 0; dt < C::DT; ++dt)
 #pragma unroll
                     for (int g4 = 0; g4 < 4; ++g4) {
-                        const int d = dt * 32 + g4 * 8 + h * 4;
+                        const int d = dt * 32 + g4 * 8 + he * 4;
                         if (d < a.hd) *reinterpret_cast<f32x4*>(op + d) = f32x4{st.o[q][dt][g4 * 4], st.o[q][dt][g4 * 4 + 1], st.o[q][dt][g4 * 4 + 2], st.o[q][dt][g4 * 4 + 3]};
                     }
-                if (h == 0) *reinterpret_cast<f32x2*>(part + R * a.hd + 2 * (r - w.row0)) = f32x2{st.m[q], l};
+                if (he == 0) *reinterpret_cast<f32x2*>(part + R * a.hd + 2 * (r - w.row0)) = f32x2{st.m[q], l};
             }
         }
         pos = start + t1;
@@ -578,7 +583,7 @@ __global__ __launch_bounds__(NW * 64, QG == 2 || HDP > 128 ? 1 : 2) void attn_pa
 template <int HDP, int NW>
 __global__ __launch_bounds__(NW * 64, 1) void attn_paged_keys_k(PagedAttn a) {
     using C = PCfg<HDP>;
-    constexpr int STAGE = 32 * (C::PK + C::PV);
+    constexpr int HALF = 32 * C::P, STAGE = 2 * HALF;
     static_assert(STAGE >= 32 * HDP * 4, "a wave's O fits its staging area");
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ float wm[NW][32], wl[NW][32];
@@ -594,23 +599,27 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_paged_keys_k(PagedAttn a) {
     const bool whole = per * 32 >= w.len;
     if (t0 >= t1 && !(whole && part == 0)) return;
     char* kb = smem + wave * STAGE;
-    char* vb = kb + 32 * C::PK;
+    char* vb = kb + HALF;
     const int srow = lane / C::CPR, sch = lane % C::CPR;
-    const int diag = a.causal && w.n > 1 ? w.len - w.n : 0x7fffffff;
     const unsigned lane_off = (unsigned)(srow * (int)a.ldkv + (sch * 8 < a.hd ? sch * 8 : 0)) * 2;
-    using Stage = PStage<HDP, 2, 1>;
-    Stage sg;
+    const int diag = a.causal && w.n > 1 ? w.len - w.n : 0x7fffffff;
+    using F = PFetch<HDP, 2, 1>;
+    F fe;
+    u32x4 kr[F::RPT], vr[F::RPT];
     unsigned next = 0;
+    int chunk = -1, ids = 0;
     auto fetch = [&](int t) {
-        next = sg.take_ids(a, w, t);
+        if (t / F::SPC != chunk) { chunk = t / F::SPC; ids = F::chunk(a, w, chunk); }
+        next = fe.take(a, w, ids, t, t1);
 #pragma unroll
-        for (int l = 0; l < 2 * Stage::RPT; ++l) sg.fetch(a, w, t, l, lane_off, 0);
-        sg.load_ids(a, w, t + NW);
+        for (int i = 0; i < F::RPT; ++i) {
+            int nk, nv;
+            bf16 *k = fe.rows(a, w, t, i, 0, nk), *v = fe.rows(a, w, t, F::RPT + i, 0, nv);
+            kr[i] = __builtin_amdgcn_raw_buffer_load_b128(__builtin_amdgcn_make_buffer_rsrc(k, 0, nk, 0x20000), lane_off, 0, 0);
+            vr[i] = __builtin_amdgcn_raw_buffer_load_b128(__builtin_amdgcn_make_buffer_rsrc(v, 0, nv, 0x20000), lane_off, 0, 0);
+        }
     };
-    if (t0 + wave < t1) {
-        sg.load_ids(a, w, t0 + wave);
-        fetch(t0 + wave);
-    }
+    if (t0 + wave < t1) fetch(t0 + wave);
     PState<HDP, 1> st;
     st.clear();
     bf16x8 qf[1][C::KS];
@@ -619,16 +628,24 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_paged_keys_k(PagedAttn a) {
     const int seen_min = min(paged_seen(a, w.len, w.n, w.row0 / a.G), w.len);
     bool dirty = false;
     for (int t = t0 + wave; t < t1; t += NW) {
-        if (!sg.full(w, t, next)) sg.blank(w, t, next, srow, 0);
-        if ((int64_t)(t + 1) * 32 > diag) dirty |= __any(sg.clean());
+        if (t * 32 + 32 > diag) {
+            bool b = false;
 #pragma unroll
-        for (int l = 0; l < 2 * Stage::RPT; ++l) sg.park(kb + srow * C::PK + sch * 16, vb + srow * C::PV + sch * 16, l, sch);
+            for (int i = 0; i < F::RPT; ++i) b |= paged_clean(vr[i]);
+            dirty |= __any(b);
+        }
+#pragma unroll
+        for (int i = 0; i < F::RPT; ++i) {
+            const int r = i * C::RPW + srow, at = r * C::P + 16 * (sch ^ C::f(r));
+            *reinterpret_cast<u32x4*>(kb + at) = kr[i];
+            *reinterpret_cast<u32x4*>(vb + at) = vr[i];
+        }
         const unsigned groups = next;
         if (t + NW < t1) fetch(t + NW);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");                          // the staged rows are read by other lanes of this wave
         __builtin_amdgcn_wave_barrier();
         int vis[1] = {min(seen[0], w.len) - (t << 5)};
-        paged_step<HDP, 1, 1>(kb, vb, qf, st, a.sl2, (t << 5) + 32 > seen_min || groups != 3u, vis, groups, [](int, int) {}, []() {}, [](int, int) {});
+        paged_step<HDP, 1, 1>(kb, vb, nullptr, qf, st, a.sl2, (t << 5) + 32 > seen_min || groups != 3u, vis, groups, [](int, int, char*) {});
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
@@ -810,7 +827,7 @@ Plan make_plan(int N, int S, int Hq, int Hkv, int hd, int max_keys) {
     const int64_t rows = (int64_t)N * G;
     Plan p = {};
     p.keys = rows <= 32 * (int64_t)S;
-    p.rows = p.keys ? 32 : 128;
+    p.rows = p.keys ? 32 : (hd > 32 && hd <= 128 && rows >= 512 * (int64_t)(S < N ? S : N) ? 256 : 128);
     p.tiles = (int)(rows / p.rows) + S;
     p.nsplit = 1;
     if (p.keys) {
@@ -823,11 +840,21 @@ Plan make_plan(int N, int S, int Hq, int Hkv, int hd, int max_keys) {
         p.ws = p.nsplit > 1 ? 4 * (int64_t)p.nsplit * N * Hq * (hd + 2) : 0;
     } else {
         // two blocks of four waves fit a CU (one where head_dim is above 128)
-        const int64_t steps = (rows / p.rows + (S < N ? S : N)) * Hkv * (((int64_t)max_keys + 63) / 64), slots = hd > 128 ? 256 : 512;
+        const int64_t steps = (rows / p.rows + (S < N ? S : N)) * Hkv * (((int64_t)max_keys + 63) / 64), slots = hd > 128 || p.rows == 256 ? 256 : 512;
         p.workers = steps / MIN_SHARE >= slots ? (int)slots : (int)((steps / MIN_SHARE + 8) / 8 * 8);
         p.ws = 16 + 16 * (int64_t)Hkv * p.tiles + 4 * (int64_t)p.workers * 2 * p.rows * (hd + 2);
     }
     return p;
+}
+
+template <int HDP, int QG, int NW, int NS>
+void launch_tile(const PagedAttn& a, const Plan& p, int ql, hipStream_t st) {
+    using C = PCfg<HDP>;
+    constexpr int smem = NS * 128 * C::P;
+    UFV_ONCE_PER_DEVICE((void)hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_tile_k<HDP, QG, NW, NS>), hipFuncAttributeMaxDynamicSharedMemorySize, smem););
+    hipLaunchKernelGGL((attn_paged_tile_k<HDP, QG, NW, NS>), dim3(p.workers), dim3(NW * 64), smem, st, a);
+    const int items = p.tiles * a.Hkv;                                                 // (a cut item's rows are spread over blocks where there are few items)
+    hipLaunchKernelGGL((attn_paged_join_tiles_k<32 * QG * NW>), dim3(items, items >= 1024 ? 8 : 32), dim3(256), 0, st, a, ql);
 }
 
 template <int HDP>
@@ -836,18 +863,16 @@ int launch(const PagedAttn& a, const Plan& p, hipStream_t st) {
     int ql = 2;
     while (ql * 4 < a.hd) ql <<= 1;
     if (p.keys) {
-        constexpr int NW = HDP > 128 ? 4 : 8, smem = NW * 32 * (C::PK + C::PV);
+        constexpr int NW = HDP > 128 ? 4 : 8, smem = NW * 64 * C::P;
         UFV_ONCE_PER_DEVICE((void)hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_keys_k<HDP, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, smem););
         hipLaunchKernelGGL((attn_paged_keys_k<HDP, NW>), dim3(p.tiles, p.nsplit, a.Hkv), dim3(NW * 64), smem, st, a);
         const int64_t rows = (int64_t)a.N * a.Hq;
         if (p.nsplit > 8) hipLaunchKernelGGL((attn_paged_join_keys_k<32 * NW, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, ql);
         else if (p.nsplit > 1) hipLaunchKernelGGL((attn_paged_join_keys_k<32 * NW, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, ql);
+    } else if (p.rows == 256) {
+        if constexpr (HDP > 32 && HDP <= 128) launch_tile<HDP, BIGQ, BIGN, 4>(a, p, ql, st);
     } else {
-        constexpr int smem = 2 * 64 * (C::PK + C::PV);
-        UFV_ONCE_PER_DEVICE((void)hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_tile_k<HDP, 1, 4>), hipFuncAttributeMaxDynamicSharedMemorySize, smem););
-        hipLaunchKernelGGL((attn_paged_tile_k<HDP, 1, 4>), dim3(p.workers), dim3(256), smem, st, a);
-        const int items = p.tiles * a.Hkv;                                             // (a cut item's rows are spread over blocks where there are few items)
-        hipLaunchKernelGGL((attn_paged_join_tiles_k<128>), dim3(items, items >= 1024 ? 8 : 32), dim3(256), 0, st, a, ql);
+        launch_tile<HDP, 1, 4, 2>(a, p, ql, st);
     }
     UFV_CHECK_LAUNCH();
     return UFV_OK;
