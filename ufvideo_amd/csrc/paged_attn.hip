@@ -13,15 +13,10 @@
 // Either may be split further over the keys by blocks (few tiles on 256 CUs); the parts leave (max, sum, un-normalised O) in 32 bits in the workspace and attn_paged_join_k adds them in order.
 #include "paged.h"
 
-#ifndef BIGQ
-#define BIGQ 1
-#define BIGN 8
-#endif
 namespace {
 
 typedef __attribute__((ext_vector_type(2))) float f32x2;
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
-
 
 struct PagedAttn {
     const bf16 *q, *pages;
@@ -31,16 +26,19 @@ struct PagedAttn {
     int N, Hq, Hkv, G, hd, causal;
     float sl2;              // scale * log2(e)
     int nsplit, tiles;      // key parts (keys kernel: upper bound) or workers (tile kernel), row tiles (upper bound)
-    float* part;            // keys kernel: [nsplit][N * Hq][hd] un-normalised O, then [nsplit][N * Hq][2] max | sum.  Tile kernel: PShare, PItem [Hkv][tiles], parts (tile_part)
+    float* part;            // keys kernel: [nsplit][N * Hq][hd] un-normalised O, then [nsplit][N * Hq][2] max | sum.  Tile kernel: PCut [nsplit], parts (tile_part)
 };
 
-// tile kernel: what the join needs to know, written by the kernel itself
-struct PShare { int64_t steps; int64_t pad; };                    // key steps of a worker's share
-struct PItem { int64_t start; int64_t cost; };                    // first step of a (kv head, row tile) in the order of all steps, its number of steps
-template <int R>
-__device__ __forceinline__ float* tile_part(const PagedAttn& a, int64_t worker, int which) {
-    char* base = reinterpret_cast<char*>(a.part) + 16 + 16 * (int64_t)a.Hkv * a.tiles;
-    return reinterpret_cast<float*>(base) + (worker * 2 + which) * ((int64_t)R * (a.hd + 2));       // R rows of hd, then R pairs (max, sum)
+// tile kernel: the item that ends in a worker's share and began in an earlier one (at most one; parts = 0: none): what the join has to know of it
+struct PCut { int w0, parts;                  // its first worker; its parts, one per worker from there on
+              int q0, row0, rows, g;          // as in PagedTile
+              int workers, pad; };            // (of worker 0: how many took a share)
+__device__ __forceinline__ PCut* tile_cut(const PagedAttn& a) { return reinterpret_cast<PCut*>(a.part); }
+// A worker leaves at most two parts: of the item that its share begins inside (0) and of the one that it ends inside (1).  A part is O as the lanes hold it -- [wave][HDP / 8][64 lanes][4], so
+// that every store is whole lines -- then R pairs (max, sum).
+template <int HDP, int R>
+__device__ __forceinline__ float* tile_part(const PagedAttn& a, int worker, int which) {
+    return a.part + (int64_t)a.nsplit * (sizeof(PCut) / 4) + ((int64_t)worker * 2 + which) * (R * (HDP + 2));
 }
 
 // what a block works on: all of it wave-uniform
@@ -117,44 +115,40 @@ struct PCfg {
     }
 };
 
-// One 32-key half tile in LDS against QG groups of 32 rows: S^T, running softmax, O^T.
-// hide: key j of the half (0 .. 31) counts for the lane's row iff j < vis (and, in 16-key groups, iff its bit of `pages` is set)
-template <int HDP, int QG>
+// what a lane keeps of its row: its part of O^T, the running maximum (log2 domain), its half of the running sum
+template <int HDP>
 struct PState {
-    f32x16 o[QG][HDP / 32];
-    float m[QG], l[QG];
+    f32x16 o[HDP / 32];
+    float m, l;
     __device__ __forceinline__ void clear() {
+        m = -INFINITY;
+        l = 0.f;
 #pragma unroll
-        for (int q = 0; q < QG; ++q) {
-            m[q] = -INFINITY;
-            l[q] = 0.f;
+        for (int i = 0; i < HDP / 32; ++i)
 #pragma unroll
-            for (int i = 0; i < HDP / 32; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[q][i][r] = 0.f;
-        }
+            for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
     }
 };
 
-// at_qk(i, n, next) runs behind the i-th of the n products of S^T: the loads of the next step (memory -> LDS at `next`) go there, a few at a time -- issued in one go they hold the wave for
+// NH half tiles of 32 keys in LDS (K rows at kb, V rows at vb) against 32 rows: S^T, running softmax, O^T.  hide: key j of the step counts for the lane's row iff j < vis and, in groups of 16
+// keys, iff its bit of `groups` is set.
+// at_qk(i, n, next) runs behind the i-th of the n products of S^T: the loads of a later step (memory -> LDS at `next`) go there, a few at a time -- issued in one go they hold the wave for
 // 1300 of the 4900 cycles of a step (the memory pipe takes one 1 KB load in 16 cycles), behind the products they cost little.  kb, vb, next do not overlap (__restrict__ lets the compiler
 // keep the loads in flight across the reads: who issues them waits for them before the barrier that publishes them).
-template <int HDP, int QG, int NH, class FQ>
-__device__ __forceinline__ void paged_step(const char* __restrict__ kb, const char* __restrict__ vb, char* __restrict__ next, const bf16x8 (&qf)[QG][HDP / 16], PState<HDP, QG>& st, float sl2, bool hide, const int (&vis)[QG], unsigned groups,
-                                           FQ&& at_qk) {
+template <int HDP, int NH, class FQ>
+__device__ __forceinline__ void paged_step(const char* __restrict__ kb, const char* __restrict__ vb, char* __restrict__ next, const bf16x8 (&qf)[HDP / 16], PState<HDP>& st, float sl2, bool hide, int vis,
+                                           unsigned groups, FQ&& at_qk) {
     using C = PCfg<HDP>;
     const int lane = threadIdx.x & 63, h = lane >> 5;
     const int k_off = C::kaddr(lane), v_off = C::vaddr(lane);
     // Left to itself the compiler puts every LDS read right in front of the matrix instruction that needs it and waits out the LDS latency 32 times a step.  The order below is pinned
     // (sched_barrier): AHEAD fragments are in flight at any time, the V reads start before the exponentials, and the second half's exponentials go between the first half's products.
     constexpr int AHEAD = 4, NR = C::KS * NH, PRE = AHEAD < NR ? AHEAD : NR;
-    f32x16 s[QG][NH];
+    f32x16 s[NH];
 #pragma unroll
-    for (int q = 0; q < QG; ++q)
+    for (int hh = 0; hh < NH; ++hh)
 #pragma unroll
-        for (int hh = 0; hh < NH; ++hh)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[q][hh][r] = 0.f;
+        for (int r = 0; r < 16; ++r) s[hh][r] = 0.f;
     {
         bf16x8 kf[PRE];
         auto read = [&](int i) { return *reinterpret_cast<const bf16x8*>(kb + (k_off ^ ((i / NH) << 5)) + (i % NH) * 32 * C::P); };
@@ -163,46 +157,38 @@ __device__ __forceinline__ void paged_step(const char* __restrict__ kb, const ch
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
-#pragma unroll
-            for (int q = 0; q < QG; ++q) s[q][i % NH] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i % PRE], qf[q][i / NH], s[q][i % NH], 0, 0, 0);
+            s[i % NH] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i % PRE], qf[i / NH], s[i % NH], 0, 0, 0);
             if (i + PRE < NR) kf[i % PRE] = read(i + PRE);
             at_qk(i, NR, next);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
     if (hide) {
-#pragma unroll
-        for (int q = 0; q < QG; ++q) {
-            const int lim = vis[q] - 4 * h;
-#pragma unroll
-            for (int hh = 0; hh < NH; ++hh)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)                          // key hh * 32 + (r & 3) + 8 (r >> 2) + 4 h
-                    s[q][hh][r] = hh * 32 + (r & 3) + 8 * (r >> 2) < lim && ((groups >> (2 * hh + (r >> 3))) & 1) ? s[q][hh][r] : -INFINITY;
-        }
-    }
-    float msub[QG];
-#pragma unroll
-    for (int q = 0; q < QG; ++q) {
-        float tmax = s[q][0][0];
+        const int lim = vis - 4 * h;
 #pragma unroll
         for (int hh = 0; hh < NH; ++hh)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, s[q][hh][r]);
-        tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64)) * sl2;
-        // the rescale of O waits until the maximum has grown by 2^6: until then the exponentials stay below 2^6 and nothing is lost
-        if (__any(tmax > st.m[q] + 6.0f)) {
-            const float mnew = fmaxf(st.m[q], tmax);
-            const float alpha = mnew == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.m[q] - mnew);
-            st.l[q] *= alpha;
-#pragma unroll
-            for (int i = 0; i < C::DT; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) st.o[q][i][r] *= alpha;
-            st.m[q] = mnew;
-        }
-        msub[q] = st.m[q] == -INFINITY ? 0.f : st.m[q];
+            for (int r = 0; r < 16; ++r)                              // key hh * 32 + (r & 3) + 8 (r >> 2) + 4 h
+                s[hh][r] = hh * 32 + (r & 3) + 8 * (r >> 2) < lim && ((groups >> (2 * hh + (r >> 3))) & 1) ? s[hh][r] : -INFINITY;
     }
+    float tmax = s[0][0];
+#pragma unroll
+    for (int hh = 0; hh < NH; ++hh)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, s[hh][r]);
+    tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64)) * sl2;
+    // the rescale of O waits until the maximum has grown by 2^6: until then the exponentials stay below 2^6 and nothing is lost
+    if (__any(tmax > st.m + 6.0f)) {
+        const float mnew = fmaxf(st.m, tmax);
+        const float alpha = mnew == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.m - mnew);
+        st.l *= alpha;
+#pragma unroll
+        for (int i = 0; i < C::DT; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) st.o[i][r] *= alpha;
+        st.m = mnew;
+    }
+    const float msub = st.m == -INFINITY ? 0.f : st.m;
     constexpr int NM = 2 * C::DT, NV = NM * NH, PREV = AHEAD < NV ? AHEAD : NV, EPM = (16 + NM - 1) / NM;      // products of a half, of the step; elements per product
     bf16x4 vf[PREV][2];
     auto readv = [&](int i, int u) {                       // product i: keys 16 (i / DT) .., dims 32 (i % DT) ..
@@ -212,48 +198,42 @@ __device__ __forceinline__ void paged_step(const char* __restrict__ kb, const ch
 #pragma unroll
     for (int i = 0; i < PREV; ++i) { vf[i][0] = readv(i, 0); vf[i][1] = readv(i, 1); }
     __builtin_amdgcn_sched_barrier(0);
-    float sum[QG];
+    float sum = 0.f;
     auto exps = [&](int hh, int r0, int r1) {
 #pragma unroll
-        for (int q = 0; q < QG; ++q)
-#pragma unroll
-            for (int r = r0; r < r1; ++r) {
-                s[q][hh][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[q][hh][r], sl2, -msub[q]));
-                sum[q] = hh == 0 && r == 0 ? s[q][hh][r] : sum[q] + s[q][hh][r];
-            }
+        for (int r = r0; r < r1; ++r) {
+            s[hh][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[hh][r], sl2, -msub));
+            sum = hh == 0 && r == 0 ? s[hh][r] : sum + s[hh][r];
+        }
     };
     exps(0, 0, 16);
-    bf16x8 pf[QG][2];
+    bf16x8 pf[2];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         if (i % NM == 0) {
 #pragma unroll
-            for (int q = 0; q < QG; ++q)
+            for (int c = 0; c < 2; ++c) {
+                float p[8];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    float p[8];
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) p[r] = s[q][i / NM][8 * c + r];
-                    pf[q][c] = pack8(p);
-                }
+                for (int r = 0; r < 8; ++r) p[r] = s[i / NM][8 * c + r];
+                pf[c] = pack8(p);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
         const bf16x8 v = __builtin_shufflevector(vf[i % PREV][0], vf[i % PREV][1], 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-        for (int q = 0; q < QG; ++q) st.o[q][i % C::DT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, pf[q][(i % NM) / C::DT], st.o[q][i % C::DT], 0, 0, 0);
+        st.o[i % C::DT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, pf[(i % NM) / C::DT], st.o[i % C::DT], 0, 0, 0);
         if (i + PREV < NV) { vf[i % PREV][0] = readv(i + PREV, 0); vf[i % PREV][1] = readv(i + PREV, 1); }
         if (NH == 2 && i < NM) exps(1, EPM * i < 16 ? EPM * i : 16, EPM * (i + 1) < 16 ? EPM * (i + 1) : 16);
         __builtin_amdgcn_sched_barrier(0);
     }
-#pragma unroll
-    for (int q = 0; q < QG; ++q) st.l[q] += sum[q];
+    st.l += sum;
 }
 
 // A key that a row does not see must not reach it even when its V row holds Inf or NaN (0 * Inf in the matrix product): among the new tokens of a causal chunk -- the only keys
 // that some rows see and others do not -- such elements are staged as zeros, and if there was one, they are added after the walk to the rows that see them (keys j0 .. j1 - 1;
 // p > 0 times Inf or NaN is Inf or NaN).
-template <int HDP, int QG>
-__device__ __forceinline__ void paged_add_bad(const PagedAttn& a, const PagedTile& w, int j0, int j1, PState<HDP, QG>& st, const int (&seen)[QG]) {
+template <int HDP>
+__device__ __forceinline__ void paged_add_bad(const PagedAttn& a, const PagedTile& w, int j0, int j1, PState<HDP>& st, int seen) {
     int h = (threadIdx.x & 63) >> 5;
     asm volatile("" : "+v"(h));                           // opaque: nothing of this path is kept in registers outside it
     for (int j = j0; j < j1; ++j) {
@@ -270,9 +250,7 @@ __device__ __forceinline__ void paged_add_bad(const PagedAttn& a, const PagedTil
                     const bf16x4 x = *reinterpret_cast<const bf16x4*>(v + d);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-#pragma unroll
-                        for (int q = 0; q < QG; ++q)
-                            if (!(fabsf((float)x[e]) < INFINITY) && j < seen[q]) st.o[q][dt][4 * g4 + e] += (float)x[e];
+                        if (!(fabsf((float)x[e]) < INFINITY) && j < seen) st.o[dt][4 * g4 + e] += (float)x[e];
                 }
             }
     }
@@ -291,22 +269,19 @@ __device__ __forceinline__ bool paged_clean(u32x4& v) {
 }
 
 // The lane's rows of the tile as B operands (lane: row l31 of the group, dims 16 ks + 8 h ..), and what they see.  Rows behind the tile's last take the last one's q; they are not stored.
-template <int HDP, int QG>
-__device__ __forceinline__ void paged_load_q(const PagedAttn& a, const PagedTile& w, int row0, bf16x8 (&qf)[QG][HDP / 16], int (&seen)[QG]) {
-    const int lane = threadIdx.x & 63, l31 = lane & 31;
+template <int HDP>
+__device__ __forceinline__ int paged_load_q(const PagedAttn& a, const PagedTile& w, int row0, bf16x8 (&qf)[HDP / 16]) {
+    const int lane = threadIdx.x & 63;
     int h = lane >> 5;
     asm volatile("" : "+v"(h));                           // opaque: the bounds of the chunks must not be kept in registers over the walk
+    const int r = min(row0 + (lane & 31), w.rows - 1), tok = r / a.G, hq = w.g * a.G + (r - tok * a.G);
+    const bf16* p = a.q + (int64_t)(w.q0 + tok) * a.ldq + hq * a.hd + h * 8;
 #pragma unroll
-    for (int q = 0; q < QG; ++q) {
-        const int r = min(row0 + 32 * q + l31, w.rows - 1), tok = r / a.G, hq = w.g * a.G + (r - tok * a.G);
-        const bf16* p = a.q + (int64_t)(w.q0 + tok) * a.ldq + hq * a.hd + h * 8;
-        seen[q] = paged_seen(a, w.len, w.n, tok);
-#pragma unroll
-        for (int ks = 0; ks < HDP / 16; ++ks) {
-            qf[q][ks] = bf16x8{0, 0, 0, 0, 0, 0, 0, 0};
-            if (ks * 16 + h * 8 < a.hd) qf[q][ks] = *reinterpret_cast<const bf16x8*>(p + ks * 16);
-        }
+    for (int ks = 0; ks < HDP / 16; ++ks) {
+        qf[ks] = bf16x8{0, 0, 0, 0, 0, 0, 0, 0};
+        if (ks * 16 + h * 8 < a.hd) qf[ks] = *reinterpret_cast<const bf16x8*>(p + ks * 16);
     }
+    return paged_seen(a, w.len, w.n, tok);
 }
 
 // Fetching NG groups of 16 keys (a step) by NWS waves.  A wave load covers RPW <= 16 rows that start at a multiple of RPW, and a page holds whole groups of 16 tokens: the page is the same
@@ -352,13 +327,19 @@ struct PFetch {
 };
 
 // ---------------------------------------------------------------------------------------------------------------------------------
-// rows split over the waves.  The work of a launch is the 64-key steps of all (kv head, row tile) items in order; every worker (block) takes an equal, contiguous share of them, so
-// that no CU waits for another whatever the lengths are: 528 equal items on 512 block slots would take two rounds, the second nearly empty.  A worker walks from where its share begins
-// inside one item to where it ends inside another; an item that lies in one share is stored at once, of the others every worker leaves a part (at most two per worker) to the join.
+// rows split over the waves.  The work of a launch is the 64-key steps of all (kv head, row tile) items in order, every item with ITEM_COST steps more for its start and end; every worker
+// (block) takes an equal, contiguous share of them, so that no CU waits for another whatever the lengths are: 528 equal items on 512 block slots would take two rounds, the second nearly
+// empty.  A worker walks from where its share begins inside one item to where it ends inside another; an item that lies in one share is stored at once, of the others every worker leaves a
+// part to the join.  The start of an item (its q rows, its first key steps) is fetched before the stores of the one before it, whose time hides it.
 // ---------------------------------------------------------------------------------------------------------------------------------
-constexpr int MIN_SHARE = 8;       // steps: a shorter share would pay more for its parts than it gains
+#ifndef MIN_SHARE_
+#define MIN_SHARE_ 8
+#define ITEM_COST_ 2
+#endif
+constexpr int MIN_SHARE = MIN_SHARE_;       // steps: a shorter share would pay more for its parts than it gains
+constexpr int ITEM_COST = ITEM_COST_;
 
-// key steps of row tile t (0: no rows; a tile that sees no key takes one, fully masked, step)
+// key steps of the row tile that begins at row0 of a slot (0: no rows; a tile that sees no key takes one, fully masked, step)
 template <int R>
 __device__ __forceinline__ int tile_steps(const PagedAttn& a, int row0, int n, int len) {
     const int rows = n * a.G;
@@ -367,33 +348,68 @@ __device__ __forceinline__ int tile_steps(const PagedAttn& a, int row0, int n, i
     return max((seen + 63) >> 6, 1);
 }
 
-template <int HDP, int QG, int NW, int NS>
-__global__ __launch_bounds__(NW * 64, QG == 2 || HDP > 128 ? 1 : 2) void attn_paged_tile_k(PagedAttn a) {
+// a / b of numbers that nearly always fit 32 bits (a 64-bit division takes 1000 cycles)
+__device__ __forceinline__ int64_t paged_div(int64_t a, int64_t b) { return ((a | b) >> 32) == 0 ? (int64_t)((unsigned)a / (unsigned)b) : a / b; }
+
+// cu_q and kv_len, a copy in LDS where they fit
+struct PSlots {
+    static constexpr int MAX = 256;
+    int cu[MAX + 1], len[MAX];
+};
+
+template <int HDP, int NW, int NS>
+__global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_tile_k(PagedAttn a) {
     using C = PCfg<HDP>;
-    constexpr int R = 32 * QG * NW, NT = NW * 64, HALF = 64 * C::P, STAGE = 2 * HALF;      // a step's K rows, its K and V rows
+    constexpr int R = 32 * NW, NT = NW * 64, HALF = 64 * C::P, STAGE = 2 * HALF;           // a step's K rows, its K and V rows
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ int dirty;
-    __shared__ int64_t scan[NW + 2];                       // wave sums | the first item's tile and its first step
+    __shared__ PSlots slots;
+    __shared__ int64_t scan[NW + 2];                       // wave sums | the first item's place: tile and slot, its first step
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = lane >> 5, l31 = lane & 31;
+    const bool cached = a.t.S <= PSlots::MAX;
+    if (cached) {
+        for (int i = tid; i <= a.t.S; i += NT) slots.cu[i] = a.t.cu_q[i];
+        for (int i = tid; i < a.t.S; i += NT) slots.len[i] = paged_len(a.t, i);
+    }
+    if (tid == 0) {
+        dirty = 0;
+        scan[NW] = scan[NW + 1] = 0;
+    }
+    __syncthreads();
+    auto cu = [&](int s) { return cached ? slots.cu[s] : a.t.cu_q[s]; };
+    auto number = [&](int s, int c) { return (int)((int64_t)c * a.G / R) + s; };           // the slot's first number, c = cu_q[s] (see paged_first_tile)
+    // tile t of slot s, which is moved on to the one whose numbers t is among: its rows, its key steps (0: a number without rows).  uni: what is read is the same in all lanes, or not
+    auto look = [&](auto&& uni, int t, int& s, PagedTile& w) {
+        int c0 = uni(cu(s)), c1 = uni(cu(s + 1));
+        while (s + 1 < a.t.S && number(s + 1, c1) <= t) {
+            ++s;
+            c0 = c1;
+            c1 = uni(cu(s + 1));
+        }
+        w.s = s;
+        w.q0 = c0;
+        w.n = c1 - c0;
+        w.row0 = (t - number(s, c0)) * R;
+        if (w.row0 < 0 || w.q0 < 0 || w.n <= 0 || w.q0 + w.n > a.N) return 0;
+        w.rows = w.n * a.G;
+        w.len = uni(cached ? slots.len[s] : paged_len(a.t, s));
+        return tile_steps<R>(a, w.row0, w.n, w.len);
+    };
 
     // ---- the share.  Every block counts the steps of one kv head's tiles (thread: a run of m tiles) and finds where its share begins.
     int64_t per_head, share, pos, end;
-    int worker, g, tile;
+    int worker, g, tile, slot;
     int64_t base;                                          // steps of the head's tiles before `tile`
     {
         const int m = (a.tiles + NT - 1) / NT, t0 = min(tid * m, a.tiles), t1 = min(t0 + m, a.tiles);
         int s = 0;
         for (int lo = 0, hi = a.t.S; lo < hi;) {           // the last slot whose numbers start at or before t0
             const int mid = (lo + hi) >> 1;
-            if (paged_first_tile<R>(a, mid) <= t0) { s = mid; lo = mid + 1; } else hi = mid;
+            if (number(mid, cu(mid)) <= t0) { s = mid; lo = mid + 1; } else hi = mid;
         }
-        auto steps = [&](int t, int& s) {
-            while (s + 1 < a.t.S && paged_first_tile<R>(a, s + 1) <= t) ++s;
-            const int q0 = a.t.cu_q[s], n = a.t.cu_q[s + 1] - q0, first = paged_first_tile<R>(a, s);
-            if (t < first || q0 < 0 || n <= 0 || q0 + n > a.N) return 0;
-            return tile_steps<R>(a, (t - first) * R, n, paged_len(a.t, s));
-        };
+        PagedTile w;
+        auto steps = [&](int t, int& s) { const int c = look([](int x) { return x; }, t, s, w); return c ? c + ITEM_COST : 0; };
         int64_t mine = 0;
         int s1 = s;
         for (int t = t0; t < t1; ++t) mine += steps(t, s1);
@@ -404,7 +420,6 @@ __global__ __launch_bounds__(NW * 64, QG == 2 || HDP > 128 ? 1 : 2) void attn_pa
             if (lane >= o) x += y;
         }
         if (lane == 63) scan[wave] = x;
-        if (tid == 0) scan[NW] = scan[NW + 1] = 0;
         __syncthreads();
         int64_t before = x - mine;
         per_head = 0;
@@ -416,63 +431,131 @@ __global__ __launch_bounds__(NW * 64, QG == 2 || HDP > 128 ? 1 : 2) void attn_pa
         const int64_t total = per_head * a.Hkv;
         int64_t workers = total / MIN_SHARE;
         workers = workers < 1 ? 1 : (workers > gridDim.x ? gridDim.x : workers);
-        share = (total + workers - 1) / workers;
+        share = max(paged_div(total + workers - 1, workers), (int64_t)1);
+        workers = paged_div(total + share - 1, share);
         // ids that differ by 8 run on one XCD: every XCD gets a contiguous run of shares, whose items share a kv head's keys in its L2
         const int per = (int)((workers + 7) >> 3), id = blockIdx.x;
         worker = (id & 7) * per + (id >> 3);
-        if ((id >> 3) >= per || worker >= workers || worker * share >= total) return;
+        if (id == 0 && tid == 0) tile_cut(a)->workers = (int)workers;
+        if ((id >> 3) >= per || worker >= workers) return;
         pos = worker * share;
         end = min(pos + share, total);
-        g = (int)(pos / per_head);
+        g = (int)paged_div(pos, per_head);
         const int64_t off = pos - g * per_head;
         if (off >= before && off < before + mine) {
             int64_t at = before;
             for (int t = t0; t < t1; ++t) {
                 const int c = steps(t, s);
-                if (off < at + c) { scan[NW] = t; scan[NW + 1] = at; break; }
+                if (off < at + c) { scan[NW] = ((int64_t)s << 32) | t; scan[NW + 1] = at; break; }
                 at += c;
             }
         }
         __syncthreads();
         tile = __builtin_amdgcn_readfirstlane((int)scan[NW]);
+        slot = __builtin_amdgcn_readfirstlane((int)(scan[NW] >> 32));
         base = scan[NW + 1];
-        if (worker == 0 && tid == 0) reinterpret_cast<PShare*>(a.part)->steps = share;
+        if (tid == 0) tile_cut(a)[worker].parts = 0;
     }
-    const int64_t begin = pos;
+    const int near = (int)min(max(share >> 3, (int64_t)1), (int64_t)1 << 20);     // a share's end that cuts less than this off an item moves to the item's end: fewer parts, and no share differs by more than 1/4
     const int srow = lane / C::CPR, sch = (lane % C::CPR) ^ C::f(wave * C::RPW + srow);  // the lane's row in a load, the chunk that belongs into its place
     const unsigned lane_off = (unsigned)(srow * (int)a.ldkv + (sch * 8 < a.hd ? sch * 8 : 0)) * 2;
-    PItem* items = reinterpret_cast<PItem*>(reinterpret_cast<char*>(a.part) + 16);
 
-    while (pos < end && g < a.Hkv) {
-        PagedTile w;
-        w.g = g;
-        const int cost = paged_tile<R>(a, tile, w) ? tile_steps<R>(a, w.row0, w.n, w.len) : 0;
-        if (cost == 0) {                                   // a number without rows
-            if (++tile >= a.tiles) { tile = 0; base = 0; ++g; }
-            continue;
+    using F = PFetch<HDP, 4, NW>;
+    constexpr int NL = F::NL, D = NS - 1;                                              // steps ahead
+    F fe;
+    PState<HDP> st;
+    bf16x8 qf[C::KS];
+    PagedTile w = {}, old = {};                                                                  // the item, the one before
+    int t0 = 0, t1 = 0, seen = 0, seen_min = 0, diag = 0;
+    bool cut = false;                                                                  // the item lies in several shares
+    int ids = 0, ids2 = 0;                                                             // of the step to be fetched next and its neighbours, of the chunk behind it
+    unsigned groups[NS];                                                               // which groups of 16 keys of the steps under way exist
+    auto dma = [&](int t, int l, char* buf) {
+        int bytes;
+        bf16* base = fe.rows(a, w, t, l, wave, bytes);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc(base, 0, bytes, 0x20000), LDS_PTR(buf + (l < NL / 2 ? 0 : HALF) + ((l % (NL / 2)) * F::PASS + wave * C::RPW) * C::P), 16, lane_off, 0, 0, 0);
+    };
+    for (bool have = false;; have = true) {
+        // ---- the next item of the share and its first loads
+        bool more = false;
+        const int old_t0 = t0;
+        const bool old_cut = cut;
+        old = w;
+        while (pos < end && g < a.Hkv) {
+            const int cost = look([](int x) { return __builtin_amdgcn_readfirstlane(x); }, tile, slot, w);
+            w.g = g;
+            if (cost) {
+                const int64_t first = g * per_head + base + ITEM_COST;                 // the unit of the item's first step
+                auto clip = [&](int64_t unit) {                                        // a share's end in steps of the item
+                    const int64_t x = unit - first;
+                    return x < near ? 0 : (cost - x < near ? cost : (int)x);
+                };
+                t0 = clip(worker * share);
+                t1 = clip(end);
+                cut = t0 != 0 || t1 != cost;
+                more = t0 < t1;
+                if (more && t0 > 0 && t1 == cost && tid == 0) {
+                    const int w0 = (int)paged_div(first + near - 1, share);            // the first whose share reaches a step of the item
+                    tile_cut(a)[worker].w0 = w0;
+                    tile_cut(a)[worker].parts = worker - w0 + 1;
+                    tile_cut(a)[worker].q0 = w.q0;
+                    tile_cut(a)[worker].row0 = w.row0;
+                    tile_cut(a)[worker].rows = w.rows;
+                    tile_cut(a)[worker].g = g;
+                }
+                pos = first + cost;
+                base += cost + ITEM_COST;
+            }
+            if (++tile >= a.tiles || base >= per_head) { tile = slot = 0; base = 0; ++g; }
+            if (more) break;
         }
-        const int64_t start = g * per_head + base;
-        const int t0 = (int)(pos - start), t1 = (int)min((int64_t)cost, end - start);
-        const bool whole = t0 == 0 && t1 == cost;
-        if (t0 == 0 && tid == 0) items[(int64_t)g * a.tiles + tile] = PItem{start, cost};
-
-        const int row0 = w.row0 + wave * 32 * QG;
-        bf16x8 qf[QG][C::KS];
-        int seen[QG];
-        paged_load_q<HDP, QG>(a, w, row0, qf, seen);
-        const int seen_min = min(paged_seen(a, w.len, w.n, min(row0, w.rows - 1) / a.G), w.len);
-        const int diag = a.causal && w.n > 1 ? w.len - w.n : 0x7fffffff;              // keys from here on are seen by some rows only
-        using F = PFetch<HDP, 4, NW>;
-        constexpr int NL = F::NL, D = NS - 1;                                          // steps ahead
-        F fe;
-        PState<HDP, QG> st;
+        if (more) {
+            seen = paged_load_q<HDP>(a, w, w.row0 + wave * 32, qf);
+            ids = F::chunk(a, w, t0 / F::SPC);
+            ids2 = F::chunk(a, w, t0 / F::SPC + 1);
+            seen_min = min(paged_seen(a, w.len, w.n, min(w.row0 + wave * 32, w.rows - 1) / a.G), w.len);
+            diag = a.causal && w.n > 1 ? w.len - w.n : 0x7fffffff;                     // keys from here on are seen by some rows only
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                if (d > 0 && (t0 + d) % F::SPC == 0) { ids = ids2; ids2 = F::chunk(a, w, (t0 + d) / F::SPC + 1); }
+                groups[d] = fe.take(a, w, ids, t0 + d, t1);
+                if (t0 + d < t1)
+#pragma unroll
+                    for (int l = 0; l < NL; ++l) dma(t0 + d, l, smem + d * STAGE);
+            }
+        }
+        // ---- O of the item before
+        if (have) {
+            int he = h;                                                                 // opaque: what follows from it (dims, bounds, addresses) must not be kept in registers over the walk
+            asm volatile("" : "+v"(he));
+            const float l = st.l + __shfl_xor(st.l, 32, 64);
+            const int r = old.row0 + wave * 32 + l31;
+            if (!old_cut) {
+                const int tok = min(r, old.rows - 1) / a.G, hq = old.g * a.G + (r - tok * a.G);
+                const float inv = l > 0.f ? 1.f / l : l;                               // l = 0: no key; NaN stays NaN
+                bf16* op = a.o + (int64_t)(old.q0 + tok) * a.ldo + hq * a.hd;
+#pragma unroll
+                for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+                    for (int g4 = 0; g4 < 4; ++g4) {
+                        const int d = dt * 32 + g4 * 8 + he * 4;
+                        if (r < old.rows && d < a.hd)
+                            *reinterpret_cast<bf16x4*>(op + d) = bf16x4{(bf16)(st.o[dt][g4 * 4] * inv), (bf16)(st.o[dt][g4 * 4 + 1] * inv), (bf16)(st.o[dt][g4 * 4 + 2] * inv), (bf16)(st.o[dt][g4 * 4 + 3] * inv)};
+                    }
+            } else {
+                float* part = tile_part<HDP, R>(a, worker, old_t0 > 0 ? 0 : 1);
+#pragma unroll
+                for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+                    for (int g4 = 0; g4 < 4; ++g4)
+                        *reinterpret_cast<f32x4*>(part + ((wave * (HDP / 8) + dt * 4 + g4) * 64 + lane) * 4) = f32x4{st.o[dt][g4 * 4], st.o[dt][g4 * 4 + 1], st.o[dt][g4 * 4 + 2], st.o[dt][g4 * 4 + 3]};
+                if (he == 0) *reinterpret_cast<f32x2*>(part + R * HDP + 2 * (wave * 32 + l31)) = f32x2{st.m, l};
+            }
+        }
+        if (!more) return;
+        // ---- the walk
         st.clear();
         bool bad = false;
-        auto dma = [&](int t, int l, char* buf) {
-            int bytes;
-            bf16* base = fe.rows(a, w, t, l, wave, bytes);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc(base, 0, bytes, 0x20000), LDS_PTR(buf + (l < NL / 2 ? 0 : HALF) + ((l % (NL / 2)) * F::PASS + wave * C::RPW) * C::P), 16, lane_off, 0, 0, 0);
-        };
         // waits until this wave's loads of step t have arrived, those of the steps behind it may still be under way (in order: at most NL of each); then takes care of elements that must
         // not meet a zero of P.  The barrier behind it publishes the step.
         auto arrived = [&](int t, char* buf) {
@@ -491,18 +574,6 @@ __global__ __launch_bounds__(NW * 64, QG == 2 || HDP > 128 ? 1 : 2) void attn_pa
                 }
             }
         };
-        int ids = F::chunk(a, w, t0 / F::SPC), ids2 = F::chunk(a, w, t0 / F::SPC + 1);    // of the step to be fetched next and its neighbours, of the chunk behind it
-        unsigned groups[NS];                                                            // which groups of 16 keys of the steps under way exist
-        __syncthreads();                                                                // the item before is done with the buffers
-        if (tid == 0) dirty = 0;
-#pragma unroll
-        for (int d = 0; d < D; ++d) {
-            if (d > 0 && (t0 + d) % F::SPC == 0) { ids = ids2; ids2 = F::chunk(a, w, (t0 + d) / F::SPC + 1); }
-            groups[d] = fe.take(a, w, ids, t0 + d, t1);
-            if (t0 + d < t1)
-#pragma unroll
-                for (int l = 0; l < NL; ++l) dma(t0 + d, l, smem + d * STAGE);
-        }
         arrived(t0, smem);
         __syncthreads();
         int cur = 0;                                                                    // the step's buffer in the ring
@@ -510,17 +581,14 @@ __global__ __launch_bounds__(NW * 64, QG == 2 || HDP > 128 ? 1 : 2) void attn_pa
             const char* kb = smem + cur * STAGE;
             char* kn = smem + (cur == 0 ? NS - 1 : cur - 1) * STAGE;                     // of step t - 1, which every wave has left: step t + D goes there
             cur = cur == NS - 1 ? 0 : cur + 1;
-            int vis[QG];
-#pragma unroll
-            for (int q = 0; q < QG; ++q) vis[q] = min(seen[q], w.len) - (t << 6);
             const unsigned keys = groups[0];
 #pragma unroll
             for (int d = 0; d + 1 < D; ++d) groups[d] = groups[d + 1];
             if ((t + D) % F::SPC == 0) { ids = ids2; ids2 = F::chunk(a, w, (t + D) / F::SPC + 1); }
             groups[D - 1] = fe.take(a, w, ids, t + D, t1);
-            const bool more = t + D < t1;
-            paged_step<HDP, QG, 2>(kb, kb + HALF, kn, qf, st, a.sl2, (t << 6) + 64 > seen_min || keys != 15u, vis, keys, [&](int i, int n, char* next) {
-                if (more) {
+            const bool fetch = t + D < t1;
+            paged_step<HDP, 2>(kb, kb + HALF, kn, qf, st, a.sl2, (t << 6) + 64 > seen_min || keys != 15u, min(seen, w.len) - (t << 6), keys, [&](int i, int n, char* next) {
+                if (fetch) {
 #pragma unroll
                     for (int l = i * NL / n; l < (i + 1) * NL / n; ++l) dma(t + D, l, next);
                 }
@@ -528,51 +596,14 @@ __global__ __launch_bounds__(NW * 64, QG == 2 || HDP > 128 ? 1 : 2) void attn_pa
             if (t + 1 < t1) arrived(t + 1, smem + cur * STAGE);
             __syncthreads();
         }
-        bad = __any(bad);
-        bad = __any(bad);
-        if (bad && lane == 0) dirty = 1;
         if ((int64_t)t1 * 64 > diag) {
+            if (bad) dirty = 1;
             __syncthreads();
-            if (dirty) paged_add_bad<HDP, QG>(a, w, max(diag, t0 << 6), min(t1 << 6, w.len), st, seen);
-        }
-        int he = h;                                                                     // opaque: what follows from it (dims, bounds, addresses) must not be kept in registers over the walk
-        asm volatile("" : "+v"(he));
-        float* part = tile_part<R>(a, worker, start <= begin ? 0 : 1);                 // the item that the share begins in, the item that it ends in
-#pragma unroll
-        for (int q = 0; q < QG; ++q) {
-            const float l = st.l[q] + __shfl_xor(st.l[q], 32, 64);
-            const int r = row0 + 32 * q + l31;
-            if (r >= w.rows) continue;
-            const int tok = r / a.G, hq = w.g * a.G + (r - tok * a.G);
-            if (whole) {
-                const float inv = l > 0.f ? 1.f / l : l;                               // l = 0: no key; NaN stays NaN
-                bf16* op = a.o + (int64_t)(w.q0 + tok) * a.ldo + hq * a.hd;
-#pragma unroll
-                for (int dt = 0; dt < C::DT; ++dt)
-#pragma unroll
-                    for (int g4 = 0; g4 < 4; ++g4) {
-                        const int d = dt * 32 + g4 * 8 + he * 4;
-                        if (d < a.hd) {
-                            const bf16x4 ov = {(bf16)(st.o[q][dt][g4 * 4] * inv), (bf16)(st.o[q][dt][g4 * 4 + 1] * inv), (bf16)(st.o[q][dt][g4 * 4 + 2] * inv), (bf16)(st.o[q][dt][g4 * 4 + 3] * inv)};
-                            *reinterpret_cast<bf16x4*>(op + d) = ov;
-                        }
-                    }
-            } else {
-                float* op = part + (int64_t)(r - w.row0) * a.hd;
-#pragma unroll
-                for (int dt = 0; dt < C::DT; ++dt)
-#pragma unroll
-                    for (int g4 = 0; g4 < 4; ++g4) {
-                        const int d = dt * 32 + g4 * 8 + he * 4;
-                        if (d < a.hd) *reinterpret_cast<f32x4*>(op + d) = f32x4{st.o[q][dt][g4 * 4], st.o[q][dt][g4 * 4 + 1], st.o[q][dt][g4 * 4 + 2], st.o[q][dt][g4 * 4 + 3]};
-                    }
-                if (he == 0) *reinterpret_cast<f32x2*>(part + R * a.hd + 2 * (r - w.row0)) = f32x2{st.m[q], l};
+            if (dirty) {
+                paged_add_bad<HDP>(a, w, max(diag, t0 << 6), min(t1 << 6, w.len), st, seen);
+                __syncthreads();
+                if (tid == 0) dirty = 0;                                                // (the next item sets it behind barriers of its own)
             }
-        }
-        pos = start + t1;
-        if (t1 == cost) {
-            base += cost;
-            if (++tile >= a.tiles || base >= per_head) { tile = 0; base = 0; ++g; }
         }
     }
 }
@@ -620,11 +651,10 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_paged_keys_k(PagedAttn a) {
         }
     };
     if (t0 + wave < t1) fetch(t0 + wave);
-    PState<HDP, 1> st;
+    PState<HDP> st;
     st.clear();
-    bf16x8 qf[1][C::KS];
-    int seen[1];
-    paged_load_q<HDP, 1>(a, w, w.row0, qf, seen);
+    bf16x8 qf[C::KS];
+    const int seen = paged_load_q<HDP>(a, w, w.row0, qf);
     const int seen_min = min(paged_seen(a, w.len, w.n, w.row0 / a.G), w.len);
     bool dirty = false;
     for (int t = t0 + wave; t < t1; t += NW) {
@@ -644,22 +674,21 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_paged_keys_k(PagedAttn a) {
         if (t + NW < t1) fetch(t + NW);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");                          // the staged rows are read by other lanes of this wave
         __builtin_amdgcn_wave_barrier();
-        int vis[1] = {min(seen[0], w.len) - (t << 5)};
-        paged_step<HDP, 1, 1>(kb, vb, nullptr, qf, st, a.sl2, (t << 5) + 32 > seen_min || groups != 3u, vis, groups, [](int, int, char*) {});
+        paged_step<HDP, 1>(kb, vb, nullptr, qf, st, a.sl2, (t << 5) + 32 > seen_min || groups != 3u, min(seen, w.len) - (t << 5), groups, [](int, int, char*) {});
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
     if (dirty)
-        for (int t = t0 + wave; t < t1; t += NW) paged_add_bad<HDP, 1>(a, w, max(diag, t << 5), min((t + 1) << 5, w.len), st, seen);
+        for (int t = t0 + wave; t < t1; t += NW) paged_add_bad<HDP>(a, w, max(diag, t << 5), min((t + 1) << 5, w.len), st, seen);
     // ---- join the waves: (m, l) and O [row][HDP] of every wave through LDS, then every thread sums columns of the rows that exist
-    const float l = st.l[0] + __shfl_xor(st.l[0], 32, 64);
-    if (h == 0) { wm[wave][l31] = st.m[0]; wl[wave][l31] = l; }
+    const float l = st.l + __shfl_xor(st.l, 32, 64);
+    if (h == 0) { wm[wave][l31] = st.m; wl[wave][l31] = l; }
     float* ob = reinterpret_cast<float*>(kb);
 #pragma unroll
     for (int dt = 0; dt < C::DT; ++dt)
 #pragma unroll
         for (int g4 = 0; g4 < 4; ++g4)
-            *reinterpret_cast<f32x4*>(ob + l31 * HDP + dt * 32 + g4 * 8 + h * 4) = f32x4{st.o[0][dt][g4 * 4], st.o[0][dt][g4 * 4 + 1], st.o[0][dt][g4 * 4 + 2], st.o[0][dt][g4 * 4 + 3]};
+            *reinterpret_cast<f32x4*>(ob + l31 * HDP + dt * 32 + g4 * 8 + h * 4) = f32x4{st.o[dt][g4 * 4], st.o[dt][g4 * 4 + 1], st.o[dt][g4 * 4 + 2], st.o[dt][g4 * 4 + 3]};
     __syncthreads();
     const int rows = min(w.rows - w.row0, 32), cols = a.hd >> 2;
     for (int i = tid; i < rows * cols; i += NW * 64) {
@@ -710,25 +739,6 @@ struct KeyParts {           // of attn_paged_keys_k
     }
     __device__ __forceinline__ const float* o(int p) const { return o0 + p * so; }
     __device__ __forceinline__ const float* ml(int p) const { return ml0 + p * sml; }
-};
-
-template <int R>
-struct TileParts {          // of attn_paged_tile_k: the workers whose shares the item touches
-    const PagedAttn* a;
-    int64_t share, start, w0;
-    int row, parts;
-    __device__ __forceinline__ bool find(const PagedAttn& aa, int item) {
-        a = &aa;
-        share = max(reinterpret_cast<const PShare*>(aa.part)->steps, (int64_t)1);
-        const PItem it = reinterpret_cast<const PItem*>(reinterpret_cast<const char*>(aa.part) + 16)[item];
-        start = it.start;
-        w0 = start / share;
-        parts = (int)((start + it.cost - 1) / share - w0) + 1;
-        return parts > 1 && w0 >= 0 && w0 + parts <= aa.nsplit;
-    }
-    __device__ __forceinline__ const float* base(int p) const { return tile_part<R>(*a, w0 + p, start <= (w0 + p) * share ? 0 : 1); }
-    __device__ __forceinline__ const float* o(int p) const { return base(p) + (int64_t)row * a->hd; }
-    __device__ __forceinline__ const float* ml(int p) const { return base(p) + R * a->hd + 2 * row; }
 };
 
 // The parts of one (row, q head), added in a fixed order with weights 2^(m_p - m) by WPR waves: lanes over quads of dims and over parts (64 / ql parts at once in a wave; ql: lanes per
@@ -797,19 +807,50 @@ __global__ __launch_bounds__(256) void attn_paged_join_keys_k(PagedAttn a, int q
     if (ps.find<UNIT>(a, n, hq, s, q0, q1)) paged_join_row<WPR>(a, ps, ql, a.o + (int64_t)n * a.ldo + hq * a.hd, red);
 }
 
-// after attn_paged_tile_k: block = (item, every gridDim.y-th group of four rows), a wave for a row; items that no share boundary cuts leave at once
-template <int R>
-__global__ __launch_bounds__(256) void attn_paged_join_tiles_k(PagedAttn a, int ql) {
-    PagedTile w;
-    w.g = blockIdx.x / a.tiles;
-    if (!paged_tile<R>(a, blockIdx.x % a.tiles, w)) return;
-    TileParts<R> ps;
-    if (!ps.find(a, blockIdx.x)) return;
-    for (int r = blockIdx.y * 4 + (threadIdx.x >> 6); r < R && w.row0 + r < w.rows; r += gridDim.y * 4) {
-        const int tok = (w.row0 + r) / a.G, hq = w.g * a.G + w.row0 + r - tok * a.G;
-        ps.row = r;
-        paged_join_row<1>(a, ps, ql, a.o + (int64_t)(w.q0 + tok) * a.ldo + hq * a.hd, nullptr);
+// after attn_paged_tile_k: blockIdx.x: the worker in whose share a cut item ends, blockIdx.y: a group of its rows.  A thread adds one quad of dims of one row over the parts, in their order,
+// with weights 2^(m_p - m); eight lanes read 128 bytes of a part as the lanes of the tile kernel left them.
+template <int HDP, int R>
+__global__ __launch_bounds__(256) void attn_paged_join_tiles_k(PagedAttn a) {
+    if ((int)blockIdx.x >= tile_cut(a)->workers) return;
+    const PCut c = tile_cut(a)[blockIdx.x];
+    if (c.parts < 2 || c.w0 < 0 || c.w0 + c.parts > a.nsplit) return;
+    const int i = blockIdx.y * 256 + threadIdx.x, quad = (i >> 3) % (HDP / 4), row = (i >> 3) / (HDP / 4) * 8 + (i & 7), r = c.row0 + row;
+    if (r >= c.rows || quad * 4 >= a.hd) return;
+    const int at = (((row >> 5) * (HDP / 8) + (quad >> 1)) * 64 + (quad & 1) * 32 + (row & 31)) * 4, at_ml = R * HDP + 2 * row;
+    // one pass with a running maximum, four parts in flight
+    float m = -INFINITY, sum = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int p0 = 0; p0 < c.parts; p0 += 4) {
+        f32x4 v[4];
+        f32x2 ml[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int p = p0 + k;
+            v[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+            ml[k] = f32x2{-INFINITY, 0.f};
+            if (p < c.parts) {
+                const float* part = tile_part<HDP, R>(a, c.w0 + p, p == 0 ? 1 : 0);
+                v[k] = *reinterpret_cast<const f32x4*>(part + at);
+                ml[k] = *reinterpret_cast<const f32x2*>(part + at_ml);
+            }
+        }
+        float mn = m;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mn = fmaxf(mn, ml[k][0]);
+        const float old = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        sum *= old;
+        o *= old;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float f = ml[k][0] == -INFINITY ? (ml[k][1] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ml[k][0] - mn);     // (a part of nothing but NaN has no maximum: its NaN stays)
+            sum += f * ml[k][1];
+            o += f * v[k];
+        }
+        m = mn;
     }
+    const float inv = sum > 0.f ? 1.f / sum : sum;
+    const int tok = r / a.G, hq = c.g * a.G + (r - tok * a.G);
+    *reinterpret_cast<bf16x4*>(a.o + (int64_t)(c.q0 + tok) * a.ldo + hq * a.hd + quad * 4) = bf16x4{(bf16)(o[0] * inv), (bf16)(o[1] * inv), (bf16)(o[2] * inv), (bf16)(o[3] * inv)};
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
@@ -840,21 +881,21 @@ Plan make_plan(int N, int S, int Hq, int Hkv, int hd, int max_keys) {
         p.ws = p.nsplit > 1 ? 4 * (int64_t)p.nsplit * N * Hq * (hd + 2) : 0;
     } else {
         // two blocks of four waves fit a CU (one where head_dim is above 128)
-        const int64_t steps = (rows / p.rows + (S < N ? S : N)) * Hkv * (((int64_t)max_keys + 63) / 64), slots = hd > 128 || p.rows == 256 ? 256 : 512;
+        const int64_t steps = (rows / p.rows + (S < N ? S : N)) * Hkv * (((int64_t)max_keys + 63) / 64 + ITEM_COST), slots = hd > 128 || p.rows == 256 ? 256 : 512;
         p.workers = steps / MIN_SHARE >= slots ? (int)slots : (int)((steps / MIN_SHARE + 8) / 8 * 8);
-        p.ws = 16 + 16 * (int64_t)Hkv * p.tiles + 4 * (int64_t)p.workers * 2 * p.rows * (hd + 2);
+        const int hdp = hd > 128 ? 256 : (hd + 31) / 32 * 32;
+        p.ws = (int64_t)p.workers * ((int64_t)sizeof(PCut) + 4 * 2 * p.rows * (hdp + 2));
     }
     return p;
 }
 
-template <int HDP, int QG, int NW, int NS>
-void launch_tile(const PagedAttn& a, const Plan& p, int ql, hipStream_t st) {
+template <int HDP, int NW, int NS>
+void launch_tile(const PagedAttn& a, const Plan& p, hipStream_t st) {
     using C = PCfg<HDP>;
     constexpr int smem = NS * 128 * C::P;
-    UFV_ONCE_PER_DEVICE((void)hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_tile_k<HDP, QG, NW, NS>), hipFuncAttributeMaxDynamicSharedMemorySize, smem););
-    hipLaunchKernelGGL((attn_paged_tile_k<HDP, QG, NW, NS>), dim3(p.workers), dim3(NW * 64), smem, st, a);
-    const int items = p.tiles * a.Hkv;                                                 // (a cut item's rows are spread over blocks where there are few items)
-    hipLaunchKernelGGL((attn_paged_join_tiles_k<32 * QG * NW>), dim3(items, items >= 1024 ? 8 : 32), dim3(256), 0, st, a, ql);
+    UFV_ONCE_PER_DEVICE((void)hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_tile_k<HDP, NW, NS>), hipFuncAttributeMaxDynamicSharedMemorySize, smem););
+    hipLaunchKernelGGL((attn_paged_tile_k<HDP, NW, NS>), dim3(p.workers), dim3(NW * 64), smem, st, a);
+    hipLaunchKernelGGL((attn_paged_join_tiles_k<HDP, 32 * NW>), dim3(p.workers, 32 * NW * (HDP / 4) / 256), dim3(256), 0, st, a);
 }
 
 template <int HDP>
@@ -870,9 +911,9 @@ int launch(const PagedAttn& a, const Plan& p, hipStream_t st) {
         if (p.nsplit > 8) hipLaunchKernelGGL((attn_paged_join_keys_k<32 * NW, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, ql);
         else if (p.nsplit > 1) hipLaunchKernelGGL((attn_paged_join_keys_k<32 * NW, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, ql);
     } else if (p.rows == 256) {
-        if constexpr (HDP > 32 && HDP <= 128) launch_tile<HDP, BIGQ, BIGN, 4>(a, p, ql, st);
+        if constexpr (HDP > 32 && HDP <= 128) launch_tile<HDP, 8, 4>(a, p, st);
     } else {
-        launch_tile<HDP, 1, 4, 2>(a, p, ql, st);
+        launch_tile<HDP, 4, 2>(a, p, st);
     }
     UFV_CHECK_LAUNCH();
     return UFV_OK;
