@@ -320,8 +320,8 @@ struct PFetch {
         if (PASS > 16)
 #pragma unroll
             for (int x = 1; x < PASS / 16; ++x) page = (wave * C::RPW) >> 4 == x ? id[((i * PASS) >> 4) + x] : page;
-        const int keys = page < 0 ? 0 : min(max(w.len - j, 0), C::RPW);
-        bytes = keys > 0 ? keys * (int)a.ldkv * 2 - ((int)a.ldkv - a.hd) * 2 : 0;       // up to the end of the last key's chunks of this head
+        const int keys = max(min((page < 0 ? 0 : w.len) - j, C::RPW), 0), ld = (int)a.ldkv;
+        bytes = max(keys * ld - (ld - a.hd), 0) * 2;                                    // up to the end of the last key's chunks of this head
         return const_cast<bf16*>(a.pages) + (((int64_t)max(page, 0) << a.t.sh) + (j & ((1 << a.t.sh) - 1))) * a.ldkv + (l < RPT ? w.g : a.Hkv + w.g) * a.hd;
     }
 };
@@ -332,12 +332,9 @@ struct PFetch {
 // empty.  A worker walks from where its share begins inside one item to where it ends inside another; an item that lies in one share is stored at once, of the others every worker leaves a
 // part to the join.  The start of an item (its q rows, its first key steps) is fetched before the stores of the one before it, whose time hides it.
 // ---------------------------------------------------------------------------------------------------------------------------------
-#ifndef MIN_SHARE_
-#define MIN_SHARE_ 8
-#define ITEM_COST_ 2
-#endif
-constexpr int MIN_SHARE = MIN_SHARE_;       // steps: a shorter share would pay more for its parts than it gains
-constexpr int ITEM_COST = ITEM_COST_;
+constexpr int ITEM_COST = 3;       // steps; 2399 causal tokens (28 / 4 heads of 128): 99 us with 2, 92 with 3, 89 with 4; 16 questions of 9 .. 83: 58, 58, 59
+constexpr int MIN_SHARE = 6;       // steps: a shorter share would pay more for its parts than it gains
+constexpr int NEAR = 4;            // see `near`
 
 // key steps of the row tile that begins at row0 of a slot (0: no rows; a tile that sees no key takes one, fully masked, step)
 template <int R>
@@ -350,6 +347,22 @@ __device__ __forceinline__ int tile_steps(const PagedAttn& a, int row0, int n, i
 
 // a / b of numbers that nearly always fit 32 bits (a 64-bit division takes 1000 cycles)
 __device__ __forceinline__ int64_t paged_div(int64_t a, int64_t b) { return ((a | b) >> 32) == 0 ? (int64_t)((unsigned)a / (unsigned)b) : a / b; }
+
+// Block-uniform values into vector registers and back: the state of the share is not used over the walk, which needs the scalar registers (held there it was spilled, and the reloads stood
+// between the products).
+template <class... T>
+__device__ __forceinline__ void to_vector(T&... x) {
+    auto one = [](auto& v) { asm volatile("" : "+v"(v)); };
+    (one(x), ...);
+}
+template <class... T>
+__device__ __forceinline__ void to_scalar(T&... x) {
+    auto one = [](auto& v) {
+        if constexpr (sizeof(v) == 8) v = (int64_t)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)v));
+        else v = __builtin_amdgcn_readfirstlane(v);
+    };
+    (one(x), ...);
+}
 
 // cu_q and kv_len, a copy in LDS where they fit
 struct PSlots {
@@ -456,7 +469,7 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_tile_k(
         base = scan[NW + 1];
         if (tid == 0) tile_cut(a)[worker].parts = 0;
     }
-    const int near = (int)min(max(share >> 3, (int64_t)1), (int64_t)1 << 20);     // a share's end that cuts less than this off an item moves to the item's end: fewer parts, and no share differs by more than 1/4
+    const int near = (int)min(max(share >> 3, (int64_t)1), (int64_t)NEAR);     // a share's end that cuts less than this off an item moves to the item's end: fewer parts, no share longer by more than 1/8
     const int srow = lane / C::CPR, sch = (lane % C::CPR) ^ C::f(wave * C::RPW + srow);  // the lane's row in a load, the chunk that belongs into its place
     const unsigned lane_off = (unsigned)(srow * (int)a.ldkv + (sch * 8 < a.hd ? sch * 8 : 0)) * 2;
 
@@ -476,6 +489,7 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_tile_k(
         __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc(base, 0, bytes, 0x20000), LDS_PTR(buf + (l < NL / 2 ? 0 : HALF) + ((l % (NL / 2)) * F::PASS + wave * C::RPW) * C::P), 16, lane_off, 0, 0, 0);
     };
     for (bool have = false;; have = true) {
+        to_scalar(pos, end, base, per_head, share, worker, tile, slot);
         // ---- the next item of the share and its first loads
         bool more = false;
         const int old_t0 = t0;
@@ -519,9 +533,8 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_tile_k(
             for (int d = 0; d < D; ++d) {
                 if (d > 0 && (t0 + d) % F::SPC == 0) { ids = ids2; ids2 = F::chunk(a, w, (t0 + d) / F::SPC + 1); }
                 groups[d] = fe.take(a, w, ids, t0 + d, t1);
-                if (t0 + d < t1)
 #pragma unroll
-                    for (int l = 0; l < NL; ++l) dma(t0 + d, l, smem + d * STAGE);
+                for (int l = 0; l < NL; ++l) dma(t0 + d, l, smem + d * STAGE);
             }
         }
         // ---- O of the item before
@@ -553,15 +566,14 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_tile_k(
             }
         }
         if (!more) return;
+        to_vector(pos, end, base, per_head, share, worker, tile, slot);
         // ---- the walk
         st.clear();
         bool bad = false;
-        // waits until this wave's loads of step t have arrived, those of the steps behind it may still be under way (in order: at most NL of each); then takes care of elements that must
-        // not meet a zero of P.  The barrier behind it publishes the step.
+        // waits until this wave's loads of step t have arrived; those of the D - 1 steps behind it may still be under way (they come in order, and behind the last step of the item the loads
+        // read nothing, but count); then takes care of elements that must not meet a zero of P.  The barrier behind it publishes the step.
         auto arrived = [&](int t, char* buf) {
-            if (D > 2 && t + 2 < t1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NL < 63 ? 2 * NL : 63) : "memory");
-            else if (D > 1 && t + 1 < t1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL < 63 ? NL : 63) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * NL < 63 ? (D - 1) * NL : 63) : "memory");
             if (t * 64 + 64 > diag) {
 #pragma unroll
                 for (int i = 0; i < NL / 2; ++i) {
@@ -586,14 +598,12 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_tile_k(
             for (int d = 0; d + 1 < D; ++d) groups[d] = groups[d + 1];
             if ((t + D) % F::SPC == 0) { ids = ids2; ids2 = F::chunk(a, w, (t + D) / F::SPC + 1); }
             groups[D - 1] = fe.take(a, w, ids, t + D, t1);
-            const bool fetch = t + D < t1;
             paged_step<HDP, 2>(kb, kb + HALF, kn, qf, st, a.sl2, (t << 6) + 64 > seen_min || keys != 15u, min(seen, w.len) - (t << 6), keys, [&](int i, int n, char* next) {
-                if (fetch) {
 #pragma unroll
-                    for (int l = i * NL / n; l < (i + 1) * NL / n; ++l) dma(t + D, l, next);
-                }
+                for (int l = i * NL / n; l < (i + 1) * NL / n; ++l) dma(t + D, l, next);
             });
             if (t + 1 < t1) arrived(t + 1, smem + cur * STAGE);
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                        // nothing is under way when the next item fills the ring
             __syncthreads();
         }
         if ((int64_t)t1 * 64 > diag) {
@@ -868,7 +878,10 @@ Plan make_plan(int N, int S, int Hq, int Hkv, int hd, int max_keys) {
     const int64_t rows = (int64_t)N * G;
     Plan p = {};
     p.keys = rows <= 32 * (int64_t)S;
-    p.rows = p.keys ? 32 : (hd > 32 && hd <= 128 && rows >= 512 * (int64_t)(S < N ? S : N) ? 256 : 128);
+    // Tiles of 256 rows (eight waves, one block a CU, a ring of four steps) fetch a key once for 256 rows, those of 128 (two or three blocks a CU, a ring of two or three) waste fewer rows and
+    // steps on short slots.  28 / 4 heads of 128, 128 | 256: 2399 tokens over 20011 757 | 679 us, 8192 causal 675 | 606, 8 x 512 over 4096 289 | 261, 16 x 150 over 2048 117 | 120,
+    // 4 x 100 over 2048 38 | 39; 14 / 2 heads of 64: 8192 tokens 412 | 443, 4 x 300 22 | 33.  Above 128 the registers of 256 rows do not fit.
+    p.rows = p.keys ? 32 : (hd > 64 && hd <= 128 && rows >= 2048 * (int64_t)(S < N ? S : N) ? 256 : 128);
     p.tiles = (int)(rows / p.rows) + S;
     p.nsplit = 1;
     if (p.keys) {
@@ -880,8 +893,8 @@ Plan make_plan(int N, int S, int Hq, int Hkv, int hd, int max_keys) {
         p.nsplit = ns < 1 ? 1 : (int)ns;
         p.ws = p.nsplit > 1 ? 4 * (int64_t)p.nsplit * N * Hq * (hd + 2) : 0;
     } else {
-        // two blocks of four waves fit a CU (one where head_dim is above 128)
-        const int64_t steps = (rows / p.rows + (S < N ? S : N)) * Hkv * (((int64_t)max_keys + 63) / 64 + ITEM_COST), slots = hd > 128 || p.rows == 256 ? 256 : 512;
+        // what fits the CUs at once: three blocks of four waves up to head_dim 64, two up to 128, one above; one block of eight
+        const int64_t steps = (rows / p.rows + (S < N ? S : N)) * Hkv * (((int64_t)max_keys + 63) / 64 + ITEM_COST), slots = hd > 128 || p.rows == 256 ? 256 : (hd <= 64 ? 768 : 512);
         p.workers = steps / MIN_SHARE >= slots ? (int)slots : (int)((steps / MIN_SHARE + 8) / 8 * 8);
         const int hdp = hd > 128 ? 256 : (hd + 31) / 32 * 32;
         p.ws = (int64_t)p.workers * ((int64_t)sizeof(PCut) + 4 * 2 * p.rows * (hdp + 2));
@@ -911,9 +924,9 @@ int launch(const PagedAttn& a, const Plan& p, hipStream_t st) {
         if (p.nsplit > 8) hipLaunchKernelGGL((attn_paged_join_keys_k<32 * NW, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, ql);
         else if (p.nsplit > 1) hipLaunchKernelGGL((attn_paged_join_keys_k<32 * NW, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, ql);
     } else if (p.rows == 256) {
-        if constexpr (HDP > 32 && HDP <= 128) launch_tile<HDP, 8, 4>(a, p, st);
+        if constexpr (HDP > 64 && HDP <= 128) launch_tile<HDP, 8, 4>(a, p, st);
     } else {
-        launch_tile<HDP, 4, 2>(a, p, st);
+        launch_tile<HDP, 4, (HDP <= 64 ? 3 : 2)>(a, p, st);
     }
     UFV_CHECK_LAUNCH();
     return UFV_OK;
