@@ -539,3 +539,10 @@ def test_two_calls_at_once():
     torch.cuda.synchronize()
     for i, o in enumerate(got):
         assert torch.equal(o, (w1, w2)[i % 2])
+
+
+@pytest.mark.parametrize("q,kv,Hq,Hkv,hd", [(190, 190, 16, 16, 8), (3, 61, 16, 16, 8), (70, 120, 8, 4, 64)])
+def test_attention_paged_many_short_items(q, kv, Hq, Hkv, hd):
+    """items of one to four steps, so many that the ends of the blocks' shares fall close behind, into and close before short items"""
+    n = 300
+    run_case([max(q - (i * 7) % 5, 1) for i in range(n)], [kv + (i * 11) % 70 for i in range(n)], Hq, Hkv, hd, 16, seed=q)

@@ -25,21 +25,21 @@ struct PagedAttn {
     PagedTable t;
     int N, Hq, Hkv, G, hd, causal;
     float sl2;              // scale * log2(e)
-    int nsplit, tiles;      // key parts (keys kernel: upper bound) or workers (tile kernel), row tiles (upper bound)
-    float* part;            // keys kernel: [nsplit][N * Hq][hd] un-normalised O, then [nsplit][N * Hq][2] max | sum.  Tile kernel: PCut [nsplit], parts (tile_part)
+    int tiles, blocks;      // row tiles (upper bound), records and workers
+    int target, sh;         // keys kernel: parts of a head that are aimed at (0: no item is cut), log2 of the keys of its step
+    float* part;            // PCut [blocks], parts (paged_part)
 };
 
-// tile kernel: the item that ends in a worker's share and began in an earlier one (at most one; parts = 0: none): what the join has to know of it
-struct PCut { int w0, parts;                  // its first worker; its parts, one per worker from there on
+// What the join has to know of an item that several blocks worked on (parts = 0: nothing to do).  A part is un-normalised O as the lanes of the tile kernel hold it --
+// [32 rows][HDP / 8][64 lanes][4], so that every store is whole lines -- then R pairs (max, sum).
+struct PCut { int first, parts;               // its first part's block; the number of its parts
               int q0, row0, rows, g;          // as in PagedTile
-              int workers, pad; };            // (of worker 0: how many took a share)
-__device__ __forceinline__ PCut* tile_cut(const PagedAttn& a) { return reinterpret_cast<PCut*>(a.part); }
-// A worker leaves at most two parts: of the item that its share begins inside (0) and of the one that it ends inside (1).  A part is O as the lanes hold it -- [wave][HDP / 8][64 lanes][4], so
-// that every store is whole lines -- then R pairs (max, sum).
+              int used, pad; };               // (of the first: how many records are valid)
+__device__ __forceinline__ PCut* paged_cut(const PagedAttn& a) { return reinterpret_cast<PCut*>(a.part); }
+template <int HDP>
+__device__ __forceinline__ int part_at(int row, int quad) { return (((row >> 5) * (HDP / 8) + (quad >> 1)) * 64 + (quad & 1) * 32 + (row & 31)) * 4; }
 template <int HDP, int R>
-__device__ __forceinline__ float* tile_part(const PagedAttn& a, int worker, int which) {
-    return a.part + (int64_t)a.nsplit * (sizeof(PCut) / 4) + ((int64_t)worker * 2 + which) * (R * (HDP + 2));
-}
+__device__ __forceinline__ float* paged_part(const PagedAttn& a, int i) { return a.part + (int64_t)a.blocks * (sizeof(PCut) / 4) + (int64_t)i * (R * (HDP + 2)); }
 
 // what a block works on: all of it wave-uniform
 struct PagedTile {
@@ -48,42 +48,8 @@ struct PagedTile {
     int g;                  // kv head
 };
 
-// Row tiles are numbered over the batch without the host knowing the lengths: slot s may use the numbers from floor(cu_q[s] * G / R) + s on; the next slot's first number is
-// never less than what slot s needs (ceil(n G / R)).  Numbers without rows leave at once.
-template <int R>
-__device__ __forceinline__ int paged_first_tile(const PagedAttn& a, int s) { return (int)((int64_t)a.t.cu_q[s] * a.G / R) + s; }
-
-template <int R>
-__device__ __forceinline__ bool paged_tile(const PagedAttn& a, int tile, PagedTile& w) {
-    const int lane = threadIdx.x & 63;
-    int b = 0;
-    for (int s0 = 0; s0 < a.t.S; s0 += 64) {
-        const int s = s0 + lane;
-        const bool mine = s < a.t.S && paged_first_tile<R>(a, s) <= tile;
-        const int c = __popcll(__ballot(mine));
-        b += c;
-        if (c < 64) break;
-    }
-    if (b == 0) return false;
-    w.s = __builtin_amdgcn_readfirstlane(b - 1);
-    w.q0 = a.t.cu_q[w.s];
-    w.n = a.t.cu_q[w.s + 1] - w.q0;
-    if (w.q0 < 0 || w.n <= 0 || w.q0 + w.n > a.N) return false;
-    w.rows = w.n * a.G;
-    w.row0 = (tile - ((int)((int64_t)w.q0 * a.G / R) + w.s)) * R;
-    w.len = paged_len(a.t, w.s);
-    return w.row0 < w.rows;
-}
-
 // keys that row r of a slot sees: tokens 0 .. paged_seen - 1
 __device__ __forceinline__ int paged_seen(const PagedAttn& a, int len, int n, int tok) { return a.causal ? max(len - n + tok + 1, 0) : len; }
-
-// the key parts of a slot of `len` tokens: every part holds the same number of UNIT-key steps, at least two of them
-template <int UNIT>
-__device__ __forceinline__ int paged_part(int len, int nsplit) {
-    const int steps = (len + UNIT - 1) / UNIT, parts = max(min(nsplit, steps / 2), 1);
-    return (steps + parts - 1) / parts;
-}
 
 __device__ __forceinline__ bf16x8 pack8(const float* p) {
     bf16x8 r;
@@ -140,7 +106,8 @@ __device__ __forceinline__ void paged_step(const char* __restrict__ kb, const ch
                                            unsigned groups, FQ&& at_qk) {
     using C = PCfg<HDP>;
     const int lane = threadIdx.x & 63, h = lane >> 5;
-    const int k_off = C::kaddr(lane), v_off = C::vaddr(lane);
+    int k_off = C::kaddr(lane), v_off = C::vaddr(lane);
+    if (NH == 1) asm volatile("" : "+v"(k_off), "+v"(v_off));      // opaque: the keys kernel holds a step of K and V in registers and has none left for the fragments' addresses
     // Left to itself the compiler puts every LDS read right in front of the matrix instruction that needs it and waits out the LDS latency 32 times a step.  The order below is pinned
     // (sched_barrier): AHEAD fragments are in flight at any time, the V reads start before the exponentials, and the second half's exponentials go between the first half's products.
     constexpr int AHEAD = 4, NR = C::KS * NH, PRE = AHEAD < NR ? AHEAD : NR;
@@ -327,28 +294,16 @@ struct PFetch {
 };
 
 // ---------------------------------------------------------------------------------------------------------------------------------
-// rows split over the waves.  The work of a launch is the 64-key steps of all (kv head, row tile) items in order, every item with ITEM_COST steps more for its start and end; every worker
-// (block) takes an equal, contiguous share of them, so that no CU waits for another whatever the lengths are: 528 equal items on 512 block slots would take two rounds, the second nearly
-// empty.  A worker walks from where its share begins inside one item to where it ends inside another; an item that lies in one share is stored at once, of the others every worker leaves a
-// part to the join.  The start of an item (its q rows, its first key steps) is fetched before the stores of the one before it, whose time hides it.
+// rows split over the waves.  The work of a launch is the 64-key steps of all (kv head, row tile) items in order, every item with ITEM_COST steps more for its start and end; every worker (block) takes an equal, contiguous share of them, so that no CU waits for another whatever the lengths are: 528 equal items on 512 block slots would take two
+// rounds, the second nearly empty.  A worker walks from where its share begins inside one item to where it ends inside another; an item that lies in one share is stored at once, of the
+// others every worker leaves a part to the join.  The start of an item (its q rows, its first keys) is fetched before the stores of the one before it, whose time hides it.
 // ---------------------------------------------------------------------------------------------------------------------------------
-constexpr int ITEM_COST = 3;       // steps; 2399 causal tokens (28 / 4 heads of 128): 99 us with 2, 92 with 3, 89 with 4; 16 questions of 9 .. 83: 58, 58, 59
-constexpr int MIN_SHARE = 6;       // steps: a shorter share would pay more for its parts than it gains
-constexpr int NEAR = 4;            // see `near`
+// ITEM_COST 2 | 3 | 4: 2399 causal tokens (28 / 4 heads of 128) 99 | 92 | 89 us, 16 questions of 9 .. 83 tokens 58 | 58 | 59
+constexpr int ITEM_COST = 3;
+constexpr int MIN_SHARE = 6;               // steps: a shorter share would pay more for its parts than it gains
+constexpr int NEAR = 4;                    // steps: a boundary that cuts less than this off an item moves to the item's end: fewer parts, no share longer by more than 1/8
 
-// key steps of the row tile that begins at row0 of a slot (0: no rows; a tile that sees no key takes one, fully masked, step)
-template <int R>
-__device__ __forceinline__ int tile_steps(const PagedAttn& a, int row0, int n, int len) {
-    const int rows = n * a.G;
-    if (row0 >= rows) return 0;
-    const int seen = min(paged_seen(a, len, n, (min(row0 + R, rows) - 1) / a.G), len);
-    return max((seen + 63) >> 6, 1);
-}
-
-// a / b of numbers that nearly always fit 32 bits (a 64-bit division takes 1000 cycles)
-__device__ __forceinline__ int64_t paged_div(int64_t a, int64_t b) { return ((a | b) >> 32) == 0 ? (int64_t)((unsigned)a / (unsigned)b) : a / b; }
-
-// Block-uniform values into vector registers and back: the state of the share is not used over the walk, which needs the scalar registers (held there it was spilled, and the reloads stood
+// Block-uniform values into vector registers and back: the state of the share is not used over an item's steps, which need the scalar registers (held there it was spilled, and the reloads stood
 // between the products).
 template <class... T>
 __device__ __forceinline__ void to_vector(T&... x) {
@@ -364,65 +319,66 @@ __device__ __forceinline__ void to_scalar(T&... x) {
     (one(x), ...);
 }
 
-// cu_q and kv_len, a copy in LDS where they fit
-struct PSlots {
-    static constexpr int MAX = 256;
+// a / b of numbers that nearly always fit 32 bits (a 64-bit division takes 1000 cycles)
+__device__ __forceinline__ int64_t paged_div(int64_t a, int64_t b) { return ((a | b) >> 32) == 0 ? (int64_t)((unsigned)a / (unsigned)b) : a / b; }
+
+struct PWalkLds {
+    static constexpr int MAX = 512;        // slots whose cu_q and kv_len have a copy here
     int cu[MAX + 1], len[MAX];
+    int64_t scan[8 + 2];                   // wave sums | the first item: slot and tile, its first step
 };
 
-template <int HDP, int NW, int NS>
-__global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_tile_k(PagedAttn a) {
-    using C = PCfg<HDP>;
-    constexpr int R = 32 * NW, NT = NW * 64, HALF = 64 * C::P, STAGE = 2 * HALF;           // a step's K rows, its K and V rows
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    __shared__ int dirty;
-    __shared__ PSlots slots;
-    __shared__ int64_t scan[NW + 2];                       // wave sums | the first item's place: tile and slot, its first step
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int h = lane >> 5, l31 = lane & 31;
-    const bool cached = a.t.S <= PSlots::MAX;
-    if (cached) {
-        for (int i = tid; i <= a.t.S; i += NT) slots.cu[i] = a.t.cu_q[i];
-        for (int i = tid; i < a.t.S; i += NT) slots.len[i] = paged_len(a.t, i);
-    }
-    if (tid == 0) {
-        dirty = 0;
-        scan[NW] = scan[NW + 1] = 0;
-    }
-    __syncthreads();
-    auto cu = [&](int s) { return cached ? slots.cu[s] : a.t.cu_q[s]; };
-    auto number = [&](int s, int c) { return (int)((int64_t)c * a.G / R) + s; };           // the slot's first number, c = cu_q[s] (see paged_first_tile)
-    // tile t of slot s, which is moved on to the one whose numbers t is among: its rows, its key steps (0: a number without rows).  uni: what is read is the same in all lanes, or not
-    auto look = [&](auto&& uni, int t, int& s, PagedTile& w) {
-        int c0 = uni(cu(s)), c1 = uni(cu(s + 1));
-        while (s + 1 < a.t.S && number(s + 1, c1) <= t) {
+template <int R, int NT>
+struct PWalk {
+    int64_t per_head, share, pos, end;     // steps of a kv head's items, of a share; the walk's place and end
+    int64_t base;                          // steps of the head's items before `tile`
+    int worker, g, tile, slot;
+
+    // row tiles of R rows are numbered over the batch without the host knowing the lengths: slot s may use the numbers from floor(cu_q[s] * G / R) + s on; the next slot's first number is
+    // never less than what slot s needs (ceil(n G / R)).  Numbers without rows have no steps.
+    __device__ static __forceinline__ int number(int G, int s, int cu) { return (int)((int64_t)cu * G / R) + s; }
+    __device__ static __forceinline__ int cu(const PagedAttn& a, const PWalkLds& m, int s) { return a.t.S <= PWalkLds::MAX ? m.cu[s] : a.t.cu_q[s]; }
+
+    // tile t of slot s, which is moved on to the one whose numbers t is among: its rows, its key steps (0: a number without rows; a tile that sees no key takes one, fully masked).
+    // UNI: t and s are the same in all lanes
+    template <bool UNI>
+    __device__ static __forceinline__ int look(const PagedAttn& a, const PWalkLds& m, int t, int& s, PagedTile& w) {
+        auto uni = [](int x) { return UNI ? __builtin_amdgcn_readfirstlane(x) : x; };
+        int c0 = uni(cu(a, m, s)), c1 = uni(cu(a, m, s + 1));
+        while (s + 1 < a.t.S && number(a.G, s + 1, c1) <= t) {
             ++s;
             c0 = c1;
-            c1 = uni(cu(s + 1));
+            c1 = uni(cu(a, m, s + 1));
         }
         w.s = s;
         w.q0 = c0;
         w.n = c1 - c0;
-        w.row0 = (t - number(s, c0)) * R;
+        w.row0 = (t - number(a.G, s, c0)) * R;
         if (w.row0 < 0 || w.q0 < 0 || w.n <= 0 || w.q0 + w.n > a.N) return 0;
         w.rows = w.n * a.G;
-        w.len = uni(cached ? slots.len[s] : paged_len(a.t, s));
-        return tile_steps<R>(a, w.row0, w.n, w.len);
-    };
+        if (w.row0 >= w.rows) return 0;
+        w.len = uni(a.t.S <= PWalkLds::MAX ? m.len[s] : paged_len(a.t, s));
+        const int seen = min(paged_seen(a, w.len, w.n, (min(w.row0 + R, w.rows) - 1) / a.G), w.len);
+        return max((seen + 63) >> 6, 1);
+    }
 
-    // ---- the share.  Every block counts the steps of one kv head's tiles (thread: a run of m tiles) and finds where its share begins.
-    int64_t per_head, share, pos, end;
-    int worker, g, tile, slot;
-    int64_t base;                                          // steps of the head's tiles before `tile`
-    {
-        const int m = (a.tiles + NT - 1) / NT, t0 = min(tid * m, a.tiles), t1 = min(t0 + m, a.tiles);
+    // Every block counts the steps of one kv head's tiles (thread: a run of them) and finds where its share begins; false: there is none.
+    __device__ __forceinline__ bool start(const PagedAttn& a, PWalkLds& m) {
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+        if (a.t.S <= PWalkLds::MAX) {
+            for (int i = tid; i <= a.t.S; i += NT) m.cu[i] = a.t.cu_q[i];
+            for (int i = tid; i < a.t.S; i += NT) m.len[i] = paged_len(a.t, i);
+        }
+        if (tid == 0) m.scan[8] = m.scan[9] = 0;
+        __syncthreads();
+        const int run = (a.tiles + NT - 1) / NT, t0 = min(tid * run, a.tiles), t1 = min(t0 + run, a.tiles);
         int s = 0;
         for (int lo = 0, hi = a.t.S; lo < hi;) {           // the last slot whose numbers start at or before t0
             const int mid = (lo + hi) >> 1;
-            if (number(mid, cu(mid)) <= t0) { s = mid; lo = mid + 1; } else hi = mid;
+            if (number(a.G, mid, cu(a, m, mid)) <= t0) { s = mid; lo = mid + 1; } else hi = mid;
         }
         PagedTile w;
-        auto steps = [&](int t, int& s) { const int c = look([](int x) { return x; }, t, s, w); return c ? c + ITEM_COST : 0; };
+        auto steps = [&](int t, int& s) { const int c = look<false>(a, m, t, s, w); return c ? c + ITEM_COST : 0; };
         int64_t mine = 0;
         int s1 = s;
         for (int t = t0; t < t1; ++t) mine += steps(t, s1);
@@ -432,15 +388,16 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_tile_k(
             const int64_t y = __shfl_up((long long)x, o, 64);
             if (lane >= o) x += y;
         }
-        if (lane == 63) scan[wave] = x;
+        if (lane == 63) m.scan[wave] = x;
         __syncthreads();
         int64_t before = x - mine;
         per_head = 0;
 #pragma unroll
-        for (int i = 0; i < NW; ++i) {
-            before += i < wave ? scan[i] : 0;
-            per_head += scan[i];
+        for (int i = 0; i < NT / 64; ++i) {
+            before += i < wave ? m.scan[i] : 0;
+            per_head += m.scan[i];
         }
+        to_scalar(per_head);
         const int64_t total = per_head * a.Hkv;
         int64_t workers = total / MIN_SHARE;
         workers = workers < 1 ? 1 : (workers > gridDim.x ? gridDim.x : workers);
@@ -449,8 +406,8 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_tile_k(
         // ids that differ by 8 run on one XCD: every XCD gets a contiguous run of shares, whose items share a kv head's keys in its L2
         const int per = (int)((workers + 7) >> 3), id = blockIdx.x;
         worker = (id & 7) * per + (id >> 3);
-        if (id == 0 && tid == 0) tile_cut(a)->workers = (int)workers;
-        if ((id >> 3) >= per || worker >= workers) return;
+        if (id == 0 && tid == 0) paged_cut(a)->used = (int)workers;
+        if ((id >> 3) >= per || worker >= workers) return false;
         pos = worker * share;
         end = min(pos + share, total);
         g = (int)paged_div(pos, per_head);
@@ -459,17 +416,69 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_tile_k(
             int64_t at = before;
             for (int t = t0; t < t1; ++t) {
                 const int c = steps(t, s);
-                if (off < at + c) { scan[NW] = ((int64_t)s << 32) | t; scan[NW + 1] = at; break; }
+                if (off < at + c) { m.scan[8] = ((int64_t)s << 32) | t; m.scan[9] = at; break; }
                 at += c;
             }
         }
         __syncthreads();
-        tile = __builtin_amdgcn_readfirstlane((int)scan[NW]);
-        slot = __builtin_amdgcn_readfirstlane((int)(scan[NW] >> 32));
-        base = scan[NW + 1];
-        if (tid == 0) tile_cut(a)[worker].parts = 0;
+        tile = (int)m.scan[8];
+        slot = (int)(m.scan[8] >> 32);
+        base = m.scan[9];
+        if (tid == 0) paged_cut(a)[worker].parts = 0;
+        return true;
     }
-    const int near = (int)min(max(share >> 3, (int64_t)1), (int64_t)NEAR);     // a share's end that cuts less than this off an item moves to the item's end: fewer parts, no share longer by more than 1/8
+
+    // the next item of the share, its steps t0 .. t1 - 1, cut: it lies in several shares; false: there is none
+    __device__ __forceinline__ bool next(const PagedAttn& a, const PWalkLds& m, PagedTile& w, int& t0, int& t1, bool& cut) {
+        to_scalar(per_head, share, pos, end, base, worker, g, tile, slot);
+        bool more = false;
+        while (!more && pos < end && g < a.Hkv) {
+            const int cost = look<true>(a, m, tile, slot, w);
+            w.g = g;
+            if (cost) {
+                const int64_t first = g * per_head + base + ITEM_COST;                      // the unit of the item's first step
+                const int near = (int)min(max(share >> 3, (int64_t)1), (int64_t)NEAR);
+                auto clip = [&](int64_t unit) {                                        // a share's end in steps of the item
+                    const int64_t x = unit - first;
+                    return x >= cost ? cost : (x < near ? 0 : (cost - x < near ? cost : (int)x));
+                };
+                t0 = clip(worker * share);
+                t1 = clip(end);
+                cut = t0 != 0 || t1 != cost;
+                more = t0 < t1;
+                if (more && t0 > 0 && t1 == cost && threadIdx.x == 0) {           // at most one item a share: its record
+                    const int w0 = (int)paged_div(first + near - 1, share);            // the first whose share reaches a step of the item
+                    PCut* c = paged_cut(a) + worker;
+                    c->first = w0;
+                    c->parts = worker - w0 + 1;
+                    c->q0 = w.q0;
+                    c->row0 = w.row0;
+                    c->rows = w.rows;
+                    c->g = g;
+                }
+                pos = first + cost;
+                base += cost + ITEM_COST;
+            }
+            if (++tile >= a.tiles || base >= per_head) { tile = slot = 0; base = 0; ++g; }
+        }
+        to_vector(per_head, share, pos, end, base, tile, slot);
+        return more;
+    }
+    __device__ __forceinline__ int me() const { return __builtin_amdgcn_readfirstlane(worker); }
+};
+
+template <int HDP, int NW, int NS>
+__global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_tile_k(PagedAttn a) {
+    using C = PCfg<HDP>;
+    constexpr int R = 32 * NW, HALF = 64 * C::P, STAGE = 2 * HALF;                         // a step's K rows, its K and V rows
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ int dirty;
+    __shared__ PWalkLds shared;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int h = lane >> 5, l31 = lane & 31;
+    if (tid == 0) dirty = 0;
+    PWalk<R, NW * 64> walk;
+    if (!walk.start(a, shared)) return;
     const int srow = lane / C::CPR, sch = (lane % C::CPR) ^ C::f(wave * C::RPW + srow);  // the lane's row in a load, the chunk that belongs into its place
     const unsigned lane_off = (unsigned)(srow * (int)a.ldkv + (sch * 8 < a.hd ? sch * 8 : 0)) * 2;
 
@@ -489,40 +498,11 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_tile_k(
         __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc(base, 0, bytes, 0x20000), LDS_PTR(buf + (l < NL / 2 ? 0 : HALF) + ((l % (NL / 2)) * F::PASS + wave * C::RPW) * C::P), 16, lane_off, 0, 0, 0);
     };
     for (bool have = false;; have = true) {
-        to_scalar(pos, end, base, per_head, share, worker, tile, slot);
         // ---- the next item of the share and its first loads
-        bool more = false;
         const int old_t0 = t0;
         const bool old_cut = cut;
         old = w;
-        while (pos < end && g < a.Hkv) {
-            const int cost = look([](int x) { return __builtin_amdgcn_readfirstlane(x); }, tile, slot, w);
-            w.g = g;
-            if (cost) {
-                const int64_t first = g * per_head + base + ITEM_COST;                 // the unit of the item's first step
-                auto clip = [&](int64_t unit) {                                        // a share's end in steps of the item
-                    const int64_t x = unit - first;
-                    return x < near ? 0 : (cost - x < near ? cost : (int)x);
-                };
-                t0 = clip(worker * share);
-                t1 = clip(end);
-                cut = t0 != 0 || t1 != cost;
-                more = t0 < t1;
-                if (more && t0 > 0 && t1 == cost && tid == 0) {
-                    const int w0 = (int)paged_div(first + near - 1, share);            // the first whose share reaches a step of the item
-                    tile_cut(a)[worker].w0 = w0;
-                    tile_cut(a)[worker].parts = worker - w0 + 1;
-                    tile_cut(a)[worker].q0 = w.q0;
-                    tile_cut(a)[worker].row0 = w.row0;
-                    tile_cut(a)[worker].rows = w.rows;
-                    tile_cut(a)[worker].g = g;
-                }
-                pos = first + cost;
-                base += cost + ITEM_COST;
-            }
-            if (++tile >= a.tiles || base >= per_head) { tile = slot = 0; base = 0; ++g; }
-            if (more) break;
-        }
+        const bool more = walk.next(a, shared, w, t0, t1, cut);
         if (more) {
             seen = paged_load_q<HDP>(a, w, w.row0 + wave * 32, qf);
             ids = F::chunk(a, w, t0 / F::SPC);
@@ -556,7 +536,7 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_tile_k(
                             *reinterpret_cast<bf16x4*>(op + d) = bf16x4{(bf16)(st.o[dt][g4 * 4] * inv), (bf16)(st.o[dt][g4 * 4 + 1] * inv), (bf16)(st.o[dt][g4 * 4 + 2] * inv), (bf16)(st.o[dt][g4 * 4 + 3] * inv)};
                     }
             } else {
-                float* part = tile_part<HDP, R>(a, worker, old_t0 > 0 ? 0 : 1);
+                float* part = paged_part<HDP, R>(a, 2 * walk.me() + (old_t0 > 0 ? 0 : 1))         /* a share's first item, its last */;
 #pragma unroll
                 for (int dt = 0; dt < C::DT; ++dt)
 #pragma unroll
@@ -566,7 +546,6 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_tile_k(
             }
         }
         if (!more) return;
-        to_vector(pos, end, base, per_head, share, worker, tile, slot);
         // ---- the walk
         st.clear();
         bool bad = false;
@@ -619,26 +598,90 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_tile_k(
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
-// keys split over the waves: no barrier until the waves' parts are joined
+// keys split over the waves: no barrier until the waves' parts are joined.  A block works on one part of an item (kv head, 32 rows of a slot); the parts are made equally long over the whole
+// batch, whatever the lengths are: `target` of them for a head, plus one for each item.  Blocks are dispatched as others end, which levels what is left.  (Equal shares as in the tile kernel
+// were tried: 138 against 131 us for 128 slots, 99 against 87 for one of 200000 tokens: the memory system is busy when the second block of a CU starts up, and the start is shorter.)
 // ---------------------------------------------------------------------------------------------------------------------------------
+// TARGET 448 | 512 | 768 | 1024 (28 / 4 heads of 128): 48 slots of 714 .. 5825 tokens 58 | 65 | 61 | 59 us, 16 of about 2200 22 | 22 | 25 | 26, one of 200000 91 | 89 | 94 | 98, one of 20000
+// with 31 of 500 23 | 23 | 27 | 28: two blocks run on a CU, and rounding up adds about half a part for each item.
+constexpr int TARGET = 448;
+constexpr int STEP_SH = 7;                 // log2 of the keys of a step: 4 waves x 32.  The shortest part is one step: one slot of 1000 tokens 10.2 us, 11.7 with two
+
+// What unit u of a head is: its tile, its keys [k0, k1) in steps, part of parts.  Every wave finds it for itself, a slot a lane, with one round of loads: sums the steps of the batch for the
+// length of a part, then the slots' units.
+__device__ __forceinline__ bool paged_unit(const PagedAttn& a, int u, PagedTile& w, int& part, int& parts, int& per) {
+    const int lane = threadIdx.x & 63;
+    int c0, n, len, tiles, steps;
+    auto load = [&](int s0) {
+        const int s = min(s0 + lane, a.t.S - 1), c1 = a.t.cu_q[s + 1];
+        c0 = a.t.cu_q[s];
+        len = paged_len(a.t, s);
+        n = c1 - c0;
+        const bool there = s0 + lane < a.t.S && c0 >= 0 && n > 0 && c1 <= a.N;
+        tiles = there ? (n * a.G + 31) >> 5 : 0;
+        steps = (int)(((unsigned)len + (1u << a.sh) - 1) >> a.sh);
+    };
+    unsigned all = 0;
+    for (int s0 = 0; s0 < a.t.S; s0 += 64) {
+        load(s0);
+        all += (unsigned)tiles * (unsigned)steps;                                      // (below 2^31 over the batch: see `sh`)
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) all += __shfl_xor(all, o, 64);
+    const int length = a.target ? max((int)((all + a.target - 1) / a.target), 1) : 1 << 30;
+    int before = 0;
+    for (int s0 = 0; s0 < a.t.S; s0 += 64) {
+        if (a.t.S > 64) load(s0);
+        const int most = max((steps + length - 1) / length, 1), p = max((steps + most - 1) / most, 1), k = max((steps + p - 1) / p, 1), mine = tiles * k;
+        int x = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(x, o, 64);
+            if (lane >= o) x += y;
+        }
+        const int c = __popcll(__ballot(before + x <= u));
+        if (c == 64) { before += __builtin_amdgcn_readlane(x, 63); continue; }
+        parts = __builtin_amdgcn_readlane(k, c);
+        per = __builtin_amdgcn_readlane(p, c);
+        w.s = s0 + c;
+        w.q0 = __builtin_amdgcn_readlane(c0, c);
+        w.n = __builtin_amdgcn_readlane(n, c);
+        w.len = __builtin_amdgcn_readlane(len, c);
+        w.rows = w.n * a.G;
+        const int r = u - before - __builtin_amdgcn_readlane(x - mine, c);
+        w.row0 = r / parts * 32;
+        part = r % parts;
+        return true;
+    }
+    return false;
+}
+
 template <int HDP, int NW>
-__global__ __launch_bounds__(NW * 64, 1) void attn_paged_keys_k(PagedAttn a) {
+__global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_keys_k(PagedAttn a) {
     using C = PCfg<HDP>;
     constexpr int HALF = 32 * C::P, STAGE = 2 * HALF;
     static_assert(STAGE >= 32 * HDP * 4, "a wave's O fits its staging area");
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ float wm[NW][32], wl[NW][32];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int h = lane >> 5, l31 = lane & 31;
-    PagedTile w;
-    const int part = blockIdx.y;
-    w.g = blockIdx.z;
-    if (!paged_tile<32>(a, blockIdx.x, w)) return;
-    const int per = paged_part<32 * NW>(w.len, a.nsplit) * NW;                         // 32-key steps of a part
-    const int kmax = paged_seen(a, w.len, w.n, (min(w.row0 + 32, w.rows) - 1) / a.G);
-    const int t0 = part * per, t1 = min(t0 + per, (kmax + 31) >> 5);
-    const bool whole = per * 32 >= w.len;
-    if (t0 >= t1 && !(whole && part == 0)) return;
+    const int h = lane >> 5, l31 = lane & 31, id = blockIdx.x;
+    PagedTile w = {};
+    int part = 0, parts = 0, per = 0;
+    w.g = id % a.Hkv;
+    const bool work = paged_unit(a, id / a.Hkv, w, part, parts, per);
+    if (a.target && tid == 0) {
+        if (id == 0) paged_cut(a)->used = gridDim.x;
+        PCut* c = paged_cut(a) + id;
+        c->first = id;
+        c->parts = work && part == 0 ? parts : 0;
+        c->q0 = w.q0;
+        c->row0 = w.row0;
+        c->rows = w.rows;
+        c->g = w.g;
+    }
+    if (!work) return;
+    const int kmax = min(paged_seen(a, w.len, w.n, (min(w.row0 + 32, w.rows) - 1) / a.G), w.len), k0 = part * per << a.sh;
+    const int t0 = k0 >> 5, t1 = min((kmax + 31) >> 5, part + 1 == parts ? 0x7fffffff : (k0 + (per << a.sh)) >> 5);       // 32-key steps
     char* kb = smem + wave * STAGE;
     char* vb = kb + HALF;
     const int srow = lane / C::CPR, sch = lane % C::CPR;
@@ -690,7 +733,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_paged_keys_k(PagedAttn a) {
     }
     if (dirty)
         for (int t = t0 + wave; t < t1; t += NW) paged_add_bad<HDP>(a, w, max(diag, t << 5), min((t + 1) << 5, w.len), st, seen);
-    // ---- join the waves: (m, l) and O [row][HDP] of every wave through LDS, then every thread sums columns of the rows that exist
+    // ---- join the waves: (m, l) and O [row][HDP] of every wave through LDS, then every thread sums quads of the rows that exist
     const float l = st.l + __shfl_xor(st.l, 32, 64);
     if (h == 0) { wm[wave][l31] = st.m; wl[wave][l31] = l; }
     float* ob = reinterpret_cast<float*>(kb);
@@ -698,11 +741,11 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_paged_keys_k(PagedAttn a) {
     for (int dt = 0; dt < C::DT; ++dt)
 #pragma unroll
         for (int g4 = 0; g4 < 4; ++g4)
-            *reinterpret_cast<f32x4*>(ob + l31 * HDP + dt * 32 + g4 * 8 + h * 4) = f32x4{st.o[dt][g4 * 4], st.o[dt][g4 * 4 + 1], st.o[dt][g4 * 4 + 2], st.o[dt][g4 * 4 + 3]};
+            *reinterpret_cast<f32x4*>(ob + l31 * HDP + (((dt * 8 + g4 * 2 + h) ^ (l31 & 7)) << 2)) = f32x4{st.o[dt][g4 * 4], st.o[dt][g4 * 4 + 1], st.o[dt][g4 * 4 + 2], st.o[dt][g4 * 4 + 3]};
     __syncthreads();
     const int rows = min(w.rows - w.row0, 32), cols = a.hd >> 2;
     for (int i = tid; i < rows * cols; i += NW * 64) {
-        const int r = i / cols, d = (i - r * cols) * 4;
+        const int r = i / cols, quad = i - r * cols;
         float m = -INFINITY;
 #pragma unroll
         for (int k = 0; k < NW; ++k) m = fmaxf(m, wm[k][r]);
@@ -712,221 +755,151 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_paged_keys_k(PagedAttn a) {
         for (int k = 0; k < NW; ++k) {
             const float f = wm[k][r] == -INFINITY ? (wl[k][r] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(wm[k][r] - m);      // (nothing but NaN has no maximum: the NaN stays)
             sum += f * wl[k][r];
-            o += f * *reinterpret_cast<const f32x4*>(smem + k * STAGE + (r * HDP + d) * 4);
+            o += f * *reinterpret_cast<const f32x4*>(smem + k * STAGE + (r * HDP + ((quad ^ (r & 7)) << 2)) * 4);
         }
-        const int tok = (w.row0 + r) / a.G, hq = w.g * a.G + (w.row0 + r - tok * a.G);
-        if (whole) {
+        if (parts == 1) {
+            const int tok = (w.row0 + r) / a.G, hq = w.g * a.G + (w.row0 + r - tok * a.G);
             const float inv = sum > 0.f ? 1.f / sum : sum;
-            *reinterpret_cast<bf16x4*>(a.o + (int64_t)(w.q0 + tok) * a.ldo + hq * a.hd + d) = bf16x4{(bf16)(o[0] * inv), (bf16)(o[1] * inv), (bf16)(o[2] * inv), (bf16)(o[3] * inv)};
+            *reinterpret_cast<bf16x4*>(a.o + (int64_t)(w.q0 + tok) * a.ldo + hq * a.hd + quad * 4) = bf16x4{(bf16)(o[0] * inv), (bf16)(o[1] * inv), (bf16)(o[2] * inv), (bf16)(o[3] * inv)};
         } else {
-            const int64_t rid = (int64_t)part * a.N * a.Hq + (int64_t)(w.q0 + tok) * a.Hq + hq;
-            *reinterpret_cast<f32x4*>(a.part + rid * a.hd + d) = o;
-            if (d == 0) {
-                float* ml = a.part + (int64_t)a.nsplit * a.N * a.Hq * a.hd + 2 * rid;
-                ml[0] = m;
-                ml[1] = sum;
-            }
+            float* dst = paged_part<HDP, 32>(a, id);
+            *reinterpret_cast<f32x4*>(dst + part_at<HDP>(r, quad)) = o;
+            if (quad == 0) *reinterpret_cast<f32x2*>(dst + 32 * HDP + 2 * r) = f32x2{m, sum};
         }
     }
 }
 
-// Where the parts of one (row, q head) are: part p has its O at o(p) and its (max, sum) at ml(p)
-struct KeyParts {           // of attn_paged_keys_k
-    const float *o0, *ml0;
-    int64_t so, sml;
-    int parts;
-    template <int UNIT>
-    __device__ __forceinline__ bool find(const PagedAttn& a, int n, int hq, int s, int q0, int q1) {
-        const int len = paged_len(a.t, s), keys = paged_part<UNIT>(len, a.nsplit) * UNIT;
-        if (keys >= len) return false;                                                 // one part: written already
-        parts = (min(paged_seen(a, len, q1 - q0, n - q0), len) + keys - 1) / keys;
-        const int64_t stride = (int64_t)a.N * a.Hq, rid = (int64_t)n * a.Hq + hq;
-        o0 = a.part + rid * a.hd;
-        ml0 = a.part + a.nsplit * stride * a.hd + 2 * rid;
-        so = stride * a.hd;
-        sml = 2 * stride;
-        return true;
-    }
-    __device__ __forceinline__ const float* o(int p) const { return o0 + p * so; }
-    __device__ __forceinline__ const float* ml(int p) const { return ml0 + p * sml; }
-};
-
-// The parts of one (row, q head), added in a fixed order with weights 2^(m_p - m) by WPR waves: lanes over quads of dims and over parts (64 / ql parts at once in a wave; ql: lanes per
-// part, the power of two from hd / 4 on), so that even 64 parts are two rounds of loads for four waves.  red: 4 x 64 quads of LDS, used where WPR = 4 waves meet.
-template <int WPR, class Parts>
-__device__ __forceinline__ void paged_join_row(const PagedAttn& a, const Parts& ps, int ql, bf16* out, float (*red)[256]) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    float m = -INFINITY;
-    for (int c = 0; c < ps.parts; c += 64) m = fmaxf(m, c + lane < ps.parts ? ps.ml(c + lane)[0] : -INFINITY);
-    m = wave_max(m);
-    const int quad = lane & (ql - 1), sub = lane / ql, np = 64 / ql;
-    const bool mine = quad * 4 < a.hd;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    float sum = 0.f;
-    for (int c = 0; c < ps.parts; c += 64) {
-        const int cn = min(ps.parts - c, 64);
-        float f = 0.f;
-        if (lane < cn) {
-            const f32x2 v = *reinterpret_cast<const f32x2*>(ps.ml(c + lane));
-            f = v[0] == -INFINITY ? (v[1] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(v[0] - m);      // (a part of nothing but NaN has no maximum: its NaN stays)
-            sum += f * v[1];
-        }
-        for (int p0 = (WPR == 4 ? wave * np : 0); p0 < cn; p0 += 4 * WPR * np) {
-            f32x4 v[4];
+// ---------------------------------------------------------------------------------------------------------------------------------
+// The join of cut items.  blockIdx.x: the item's record.  A thread adds one quad of dims of one row over the parts, in their order, with weights 2^(m_p - m); eight lanes
+// read 128 bytes of a part as the lanes of the tile kernel left them.  PG = 4 (few rows, many parts: the keys kernel): each wave takes a quarter of the parts, they meet in LDS.
+// ---------------------------------------------------------------------------------------------------------------------------------
+template <int HDP, int R, int PG>
+__global__ __launch_bounds__(256) void attn_paged_join_k(PagedAttn a) {
+    constexpr int T = 256 / PG, U = PG > 1 ? 8 : 4;                                    // threads over (row, quad); parts in flight
+    __shared__ float red[PG > 1 ? PG - 1 : 1][6][64];
+    if ((int)blockIdx.x >= paged_cut(a)->used) return;
+    const PCut c = paged_cut(a)[blockIdx.x];
+    const int step = PG > 1 ? a.Hkv : 1;                                                // keys kernel: the units of a head; tile kernel: the workers, two parts each
+    if (c.parts < 2 || c.first < 0 || c.first + (c.parts - 1) * step >= a.blocks) return;
+    const int pg = PG > 1 ? threadIdx.x / T : 0, per = (c.parts + PG - 1) / PG, pb = min(pg * per, c.parts), pe = min(pb + per, c.parts);
+    for (int i0 = blockIdx.y * T; i0 < R * (HDP / 4); i0 += gridDim.y * T) {
+        const int i = i0 + threadIdx.x % T, quad = (i >> 3) % (HDP / 4), row = (i >> 3) / (HDP / 4) * 8 + (i & 7), r = c.row0 + row;
+        if (c.row0 + (i0 >> 3) / (HDP / 4) * 8 >= c.rows) return;                      // (the same for all threads)
+        const bool mine = r < c.rows && quad * 4 < a.hd;
+        const int at = part_at<HDP>(row, quad), at_ml = R * HDP + 2 * row;
+        // one pass with a running maximum, U parts in flight
+        float m = -INFINITY, sum = 0.f;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        auto add = [&](float mp, float lp, const f32x4& op, float mn) {
+            const float f = mp == -INFINITY ? (lp == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(mp - mn);               // (a part of nothing but NaN has no maximum: its NaN stays)
+            sum += f * lp;
+            o += f * op;
+        };
+        auto raise = [&](float mn) {
+            const float f = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            sum *= f;
+            o *= f;
+            m = mn;
+        };
+        for (int p0 = mine ? pb : pe; p0 < pe; p0 += U) {
+            f32x4 v[U];
+            f32x2 ml[U];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int p = p0 + k * WPR * np + sub;
+            for (int k = 0; k < U; ++k) {
+                const int p = p0 + k;
                 v[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (mine && p < cn) v[k] = *reinterpret_cast<const f32x4*>(ps.o(c + p) + quad * 4);
+                ml[k] = f32x2{-INFINITY, 0.f};
+                if (p < pe) {
+                    const float* part = paged_part<HDP, R>(a, PG > 1 ? c.first + p * step : 2 * (c.first + p) + (p == 0 ? 1 : 0));
+                    v[k] = *reinterpret_cast<const f32x4*>(part + at);
+                    ml[k] = *reinterpret_cast<const f32x2*>(part + at_ml);
+                }
             }
+            float mn = m;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int p = p0 + k * WPR * np + sub;
-                const float fp = __shfl(f, p < cn ? p : 0, 64);
-                if (p < cn) o += fp * v[k];
-            }
+            for (int k = 0; k < U; ++k) mn = fmaxf(mn, ml[k][0]);
+            raise(mn);
+#pragma unroll
+            for (int k = 0; k < U; ++k) add(ml[k][0], ml[k][1], v[k], m);
         }
-    }
-    sum = wave_sum(sum);
-    const float inv = sum > 0.f ? 1.f / sum : sum;
-    for (int d = ql; d < 64; d <<= 1)
+        if constexpr (PG > 1) {
+            const int lane = threadIdx.x % T;
+            __syncthreads();
+            if (pg > 0) {
+                red[pg - 1][0][lane] = m;
+                red[pg - 1][1][lane] = sum;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], d, 64);
-    if (WPR == 4) {
-        *reinterpret_cast<f32x4*>(&red[wave][lane * 4]) = o;
-        __syncthreads();
-        if (wave) return;
+                for (int e = 0; e < 4; ++e) red[pg - 1][2 + e][lane] = o[e];
+            }
+            __syncthreads();
+            if (pg > 0) continue;
 #pragma unroll
-        for (int k = 1; k < 4; ++k) o += *reinterpret_cast<const f32x4*>(&red[k][lane * 4]);
-    }
-    if (sub == 0 && mine) *reinterpret_cast<bf16x4*>(out + quad * 4) = bf16x4{(bf16)(o[0] * inv), (bf16)(o[1] * inv), (bf16)(o[2] * inv), (bf16)(o[3] * inv)};
-}
-
-// after attn_paged_keys_k: WPR = 4: a block for one (row, q head) (few rows, many parts); WPR = 1: four to a block
-template <int UNIT, int WPR>
-__global__ __launch_bounds__(256) void attn_paged_join_keys_k(PagedAttn a, int ql) {
-    __shared__ float red[4][256];
-    const int64_t id = WPR == 4 ? blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (id >= (int64_t)a.N * a.Hq) return;
-    const int n = __builtin_amdgcn_readfirstlane((int)(id / a.Hq)), hq = __builtin_amdgcn_readfirstlane((int)(id % a.Hq));
-    const int s = paged_slot_of_row(a.t.cu_q, a.t.S, n);
-    if (s >= a.t.S) return;
-    const int q0 = a.t.cu_q[s], q1 = a.t.cu_q[s + 1];
-    if (n < q0 || n >= q1 || q0 < 0 || q1 > a.N) return;
-    KeyParts ps;
-    if (ps.find<UNIT>(a, n, hq, s, q0, q1)) paged_join_row<WPR>(a, ps, ql, a.o + (int64_t)n * a.ldo + hq * a.hd, red);
-}
-
-// after attn_paged_tile_k: blockIdx.x: the worker in whose share a cut item ends, blockIdx.y: a group of its rows.  A thread adds one quad of dims of one row over the parts, in their order,
-// with weights 2^(m_p - m); eight lanes read 128 bytes of a part as the lanes of the tile kernel left them.
-template <int HDP, int R>
-__global__ __launch_bounds__(256) void attn_paged_join_tiles_k(PagedAttn a) {
-    if ((int)blockIdx.x >= tile_cut(a)->workers) return;
-    const PCut c = tile_cut(a)[blockIdx.x];
-    if (c.parts < 2 || c.w0 < 0 || c.w0 + c.parts > a.nsplit) return;
-    const int i = blockIdx.y * 256 + threadIdx.x, quad = (i >> 3) % (HDP / 4), row = (i >> 3) / (HDP / 4) * 8 + (i & 7), r = c.row0 + row;
-    if (r >= c.rows || quad * 4 >= a.hd) return;
-    const int at = (((row >> 5) * (HDP / 8) + (quad >> 1)) * 64 + (quad & 1) * 32 + (row & 31)) * 4, at_ml = R * HDP + 2 * row;
-    // one pass with a running maximum, four parts in flight
-    float m = -INFINITY, sum = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int p0 = 0; p0 < c.parts; p0 += 4) {
-        f32x4 v[4];
-        f32x2 ml[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int p = p0 + k;
-            v[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-            ml[k] = f32x2{-INFINITY, 0.f};
-            if (p < c.parts) {
-                const float* part = tile_part<HDP, R>(a, c.w0 + p, p == 0 ? 1 : 0);
-                v[k] = *reinterpret_cast<const f32x4*>(part + at);
-                ml[k] = *reinterpret_cast<const f32x2*>(part + at_ml);
+            for (int k = 0; k < PG - 1; ++k) {
+                const float mk = red[k][0][lane];
+                raise(fmaxf(m, mk));
+                add(mk, red[k][1][lane], f32x4{red[k][2][lane], red[k][3][lane], red[k][4][lane], red[k][5][lane]}, m);
             }
         }
-        float mn = m;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) mn = fmaxf(mn, ml[k][0]);
-        const float old = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-        sum *= old;
-        o *= old;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float f = ml[k][0] == -INFINITY ? (ml[k][1] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ml[k][0] - mn);     // (a part of nothing but NaN has no maximum: its NaN stays)
-            sum += f * ml[k][1];
-            o += f * v[k];
-        }
-        m = mn;
+        if (!mine) continue;
+        const float inv = sum > 0.f ? 1.f / sum : sum;
+        const int tok = r / a.G, hq = c.g * a.G + (r - tok * a.G);
+        *reinterpret_cast<bf16x4*>(a.o + (int64_t)(c.q0 + tok) * a.ldo + hq * a.hd + quad * 4) = bf16x4{(bf16)(o[0] * inv), (bf16)(o[1] * inv), (bf16)(o[2] * inv), (bf16)(o[3] * inv)};
     }
-    const float inv = sum > 0.f ? 1.f / sum : sum;
-    const int tok = r / a.G, hq = c.g * a.G + (r - tok * a.G);
-    *reinterpret_cast<bf16x4*>(a.o + (int64_t)(c.q0 + tok) * a.ldo + hq * a.hd + quad * 4) = bf16x4{(bf16)(o[0] * inv), (bf16)(o[1] * inv), (bf16)(o[2] * inv), (bf16)(o[3] * inv)};
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
 struct Plan {
     bool keys;              // keys split over the waves (else rows)
-    int rows, tiles;
-    int nsplit;             // keys kernel: parts
-    int workers;            // tile kernel: blocks
+    int rows, tiles;        // of a tile; upper bound of their number
+    int blocks, target, sh; // as in PagedAttn
     int64_t ws;             // bytes
 };
 
 // N, S: packed rows and slots; the lengths are on the device, the choice is made from the sizes alone.  A slot has N / S rows on average.
 Plan make_plan(int N, int S, int Hq, int Hkv, int hd, int max_keys) {
-    const int G = Hq / Hkv;
+    const int G = Hq / Hkv, hdp = hd > 128 ? 256 : (hd + 31) / 32 * 32, used = S < N ? S : N;
     const int64_t rows = (int64_t)N * G;
     Plan p = {};
     p.keys = rows <= 32 * (int64_t)S;
     // Tiles of 256 rows (eight waves, one block a CU, a ring of four steps) fetch a key once for 256 rows, those of 128 (two or three blocks a CU, a ring of two or three) waste fewer rows and
     // steps on short slots.  28 / 4 heads of 128, 128 | 256: 2399 tokens over 20011 757 | 679 us, 8192 causal 675 | 606, 8 x 512 over 4096 289 | 261, 16 x 150 over 2048 117 | 120,
     // 4 x 100 over 2048 38 | 39; 14 / 2 heads of 64: 8192 tokens 412 | 443, 4 x 300 22 | 33.  Above 128 the registers of 256 rows do not fit.
-    p.rows = p.keys ? 32 : (hd > 64 && hd <= 128 && rows >= 2048 * (int64_t)(S < N ? S : N) ? 256 : 128);
+    p.rows = p.keys ? 32 : (hd > 64 && hd <= 128 && rows >= 2048 * (int64_t)used ? 256 : 128);
     p.tiles = (int)(rows / p.rows) + S;
-    p.nsplit = 1;
     if (p.keys) {
-        const int unit = 32 * (hd > 128 ? 4 : 8);
-        const int64_t blocks = (int64_t)(N < S ? N : S) * Hkv, steps = ((int64_t)max_keys + unit - 1) / unit;
-        int64_t ns = (256 + blocks - 1) / blocks;
-        if (ns > steps / 2) ns = steps / 2;
-        if (ns > 64) ns = 64;
-        p.nsplit = ns < 1 ? 1 : (int)ns;
-        p.ws = p.nsplit > 1 ? 4 * (int64_t)p.nsplit * N * Hq * (hd + 2) : 0;
+        p.target = max_keys > 4 << STEP_SH ? (TARGET + Hkv - 1) / Hkv : 0;                // (333 tokens in one block 10.3 us, in three and joined 10.2)
+        p.blocks = (p.target + p.tiles) * Hkv;
+        for (p.sh = STEP_SH; (int64_t)p.tiles * ((max_keys >> p.sh) + 1) > 0x7fffffff;) ++p.sh;
+        p.ws = p.target ? (int64_t)p.blocks * ((int64_t)sizeof(PCut) + 4 * 32 * (hdp + 2)) : 0;
     } else {
         // what fits the CUs at once: three blocks of four waves up to head_dim 64, two up to 128, one above; one block of eight
-        const int64_t steps = (rows / p.rows + (S < N ? S : N)) * Hkv * (((int64_t)max_keys + 63) / 64 + ITEM_COST), slots = hd > 128 || p.rows == 256 ? 256 : (hd <= 64 ? 768 : 512);
-        p.workers = steps / MIN_SHARE >= slots ? (int)slots : (int)((steps / MIN_SHARE + 8) / 8 * 8);
-        const int hdp = hd > 128 ? 256 : (hd + 31) / 32 * 32;
-        p.ws = (int64_t)p.workers * ((int64_t)sizeof(PCut) + 4 * 2 * p.rows * (hdp + 2));
+        const int slots = hd > 128 || p.rows == 256 ? 256 : (hd <= 64 ? 768 : 512);
+        const int64_t steps = (rows / p.rows + used) * Hkv * (((int64_t)max_keys + 63) / 64 + ITEM_COST);
+        p.blocks = steps / MIN_SHARE >= slots ? slots : (int)((steps / MIN_SHARE + 8) / 8 * 8);
+        p.ws = (int64_t)p.blocks * ((int64_t)sizeof(PCut) + 2 * 4 * p.rows * (hdp + 2));
     }
     return p;
 }
 
 template <int HDP, int NW, int NS>
-void launch_tile(const PagedAttn& a, const Plan& p, hipStream_t st) {
-    using C = PCfg<HDP>;
-    constexpr int smem = NS * 128 * C::P;
+void launch_tile(const PagedAttn& a, hipStream_t st) {
+    constexpr int smem = NS * 128 * PCfg<HDP>::P;
     UFV_ONCE_PER_DEVICE((void)hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_tile_k<HDP, NW, NS>), hipFuncAttributeMaxDynamicSharedMemorySize, smem););
-    hipLaunchKernelGGL((attn_paged_tile_k<HDP, NW, NS>), dim3(p.workers), dim3(NW * 64), smem, st, a);
-    hipLaunchKernelGGL((attn_paged_join_tiles_k<HDP, 32 * NW>), dim3(p.workers, 32 * NW * (HDP / 4) / 256), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_paged_tile_k<HDP, NW, NS>), dim3(a.blocks), dim3(NW * 64), smem, st, a);
+    hipLaunchKernelGGL((attn_paged_join_k<HDP, 32 * NW, 1>), dim3(a.blocks, 32 * NW * (HDP / 4) / 256), dim3(256), 0, st, a);
 }
 
 template <int HDP>
 int launch(const PagedAttn& a, const Plan& p, hipStream_t st) {
-    using C = PCfg<HDP>;
-    int ql = 2;
-    while (ql * 4 < a.hd) ql <<= 1;
     if (p.keys) {
-        constexpr int NW = HDP > 128 ? 4 : 8, smem = NW * 64 * C::P;
+        constexpr int NW = 4, smem = NW * 64 * PCfg<HDP>::P;
         UFV_ONCE_PER_DEVICE((void)hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_keys_k<HDP, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, smem););
-        hipLaunchKernelGGL((attn_paged_keys_k<HDP, NW>), dim3(p.tiles, p.nsplit, a.Hkv), dim3(NW * 64), smem, st, a);
-        const int64_t rows = (int64_t)a.N * a.Hq;
-        if (p.nsplit > 8) hipLaunchKernelGGL((attn_paged_join_keys_k<32 * NW, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, ql);
-        else if (p.nsplit > 1) hipLaunchKernelGGL((attn_paged_join_keys_k<32 * NW, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, ql);
+        hipLaunchKernelGGL((attn_paged_keys_k<HDP, NW>), dim3(a.blocks), dim3(NW * 64), smem, st, a);
+        if (p.target) hipLaunchKernelGGL((attn_paged_join_k<HDP, 32, 4>), dim3(a.blocks, HDP / 32), dim3(256), 0, st, a);
     } else if (p.rows == 256) {
-        if constexpr (HDP > 64 && HDP <= 128) launch_tile<HDP, 8, 4>(a, p, st);
+        if constexpr (HDP > 64 && HDP <= 128) launch_tile<HDP, 8, 4>(a, st);
     } else {
-        launch_tile<HDP, 4, (HDP <= 64 ? 3 : 2)>(a, p, st);
+        launch_tile<HDP, 4, (HDP <= 64 ? 3 : 2)>(a, st);
     }
     UFV_CHECK_LAUNCH();
     return UFV_OK;
@@ -951,7 +924,7 @@ extern "C" int ufv_attention_paged(const void* q, int64_t ldq, void* o, int64_t 
     UFV_REQUIRE(ldkv >= 2 * (int64_t)Hkv * hd && ldkv < 1 << 24 && (N == 1 || (ldq >= (int64_t)Hq * hd && ldo >= (int64_t)Hq * hd)), "ufv_attention_paged: a row pitch is out of range");
     UFV_REQUIRE((int64_t)N * Hq < 0x7fffffff && S < 1 << 24, "ufv_attention_paged: too many rows or slots (N=%d S=%d)", N, S);
     const Plan p = make_plan(N, S, Hq, Hkv, hd, max_pages << paged_log2(page));
-    UFV_REQUIRE((int64_t)p.tiles * Hkv < 0x7fffffff && Hkv < 65536, "ufv_attention_paged: too many row tiles (N=%d S=%d)", N, S);
+    UFV_REQUIRE(((int64_t)p.tiles + p.target) * Hkv < 0x7fffffff && Hkv < 65536, "ufv_attention_paged: too many row tiles (N=%d S=%d)", N, S);
     UFV_REQUIRE(p.ws == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= p.ws), "ufv_attention_paged: a 16-byte aligned workspace of %lld bytes is needed (%lld given)", (long long)p.ws,
                 (long long)ws_bytes);
     PagedAttn a;
@@ -960,7 +933,7 @@ extern "C" int ufv_attention_paged(const void* q, int64_t ldq, void* o, int64_t 
     a.t = PagedTable{block_table, ld_table, max_pages, cu_q, kv_len, S, n_pages, paged_log2(page)};
     a.N = N; a.Hq = Hq; a.Hkv = Hkv; a.G = Hq / Hkv; a.hd = hd; a.causal = causal != 0;
     a.sl2 = scale * 1.4426950408889634f;
-    a.nsplit = p.keys ? p.nsplit : p.workers; a.tiles = p.tiles; a.part = (float*)ws;
+    a.tiles = p.tiles; a.blocks = p.blocks; a.target = p.target; a.sh = p.sh; a.part = (float*)ws;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (hd <= 32) return launch<32>(a, p, st);
     if (hd <= 64) return launch<64>(a, p, st);
