@@ -300,7 +300,7 @@ struct PFetch {
 // ---------------------------------------------------------------------------------------------------------------------------------
 // ITEM_COST 2 | 3 | 4: 2399 causal tokens (28 / 4 heads of 128) 99 | 92 | 89 us, 16 questions of 9 .. 83 tokens 58 | 58 | 59
 constexpr int ITEM_COST = 3;
-constexpr int MIN_SHARE = 6;               // steps: a shorter share would pay more for its parts than it gains
+constexpr int MIN_SHARE = 4;               // steps: the shortest item.  6 | 4: 40 causal tokens 18.5 | 13.0 us, 600 32 | 29, 2399 94 | 93
 constexpr int NEAR = 4;                    // steps: a boundary that cuts less than this off an item moves to the item's end: fewer parts, no share longer by more than 1/8
 
 // Block-uniform values into vector registers and back: the state of the share is not used over an item's steps, which need the scalar registers (held there it was spilled, and the reloads stood
@@ -862,9 +862,10 @@ Plan make_plan(int N, int S, int Hq, int Hkv, int hd, int max_keys) {
     Plan p = {};
     p.keys = rows <= 32 * (int64_t)S;
     // Tiles of 256 rows (eight waves, one block a CU, a ring of four steps) fetch a key once for 256 rows, those of 128 (two or three blocks a CU, a ring of two or three) waste fewer rows and
-    // steps on short slots.  28 / 4 heads of 128, 128 | 256: 2399 tokens over 20011 757 | 679 us, 8192 causal 675 | 606, 8 x 512 over 4096 289 | 261, 16 x 150 over 2048 117 | 120,
-    // 4 x 100 over 2048 38 | 39; 14 / 2 heads of 64: 8192 tokens 412 | 443, 4 x 300 22 | 33.  Above 128 the registers of 256 rows do not fit.
-    p.rows = p.keys ? 32 : (hd > 64 && hd <= 128 && rows >= 2048 * (int64_t)used ? 256 : 128);
+    // steps on short slots and sequences.  28 / 4 heads of 128, 128 | 256: 2399 tokens over 20011 757 | 679 us, 8192 causal 675 | 606, 8 x 512 over 4096 289 | 261, 16 x 150 over 2048
+    // 117 | 120, 4 x 100 over 2048 38 | 39, 8 x 600 causal 69 | 76, 300 causal 22 | 27; 14 / 2 heads of 64: 8192 tokens 412 | 443, 4 x 300 22 | 33.  Above 128 the registers of 256 rows do
+    // not fit.
+    p.rows = p.keys ? 32 : (hd > 64 && hd <= 128 && rows >= 2048 * (int64_t)used && max_keys >= 2048 ? 256 : 128);
     p.tiles = (int)(rows / p.rows) + S;
     if (p.keys) {
         p.target = max_keys > 4 << STEP_SH ? (TARGET + Hkv - 1) / Hkv : 0;                // (333 tokens in one block 10.3 us, in three and joined 10.2)
