@@ -48,6 +48,11 @@ struct PagedTile {
     int g;                  // kv head
 };
 
+// Row tiles of R rows are numbered over the batch without the host knowing the lengths: slot s may use the numbers from floor(cu_q[s] * G / R) + s on; the next slot's first number is never
+// less than what slot s needs (ceil(n G / R)).  Numbers without rows have no work.
+template <int R>
+__device__ __forceinline__ int paged_number(int G, int s, int cu) { return (int)((int64_t)cu * G / R) + s; }
+
 // keys that row r of a slot sees: tokens 0 .. paged_seen - 1
 __device__ __forceinline__ int paged_seen(const PagedAttn& a, int len, int n, int tok) { return a.causal ? max(len - n + tok + 1, 0) : len; }
 
@@ -334,9 +339,7 @@ struct PWalk {
     int64_t base;                          // steps of the head's items before `tile`
     int worker, g, tile, slot;
 
-    // row tiles of R rows are numbered over the batch without the host knowing the lengths: slot s may use the numbers from floor(cu_q[s] * G / R) + s on; the next slot's first number is
-    // never less than what slot s needs (ceil(n G / R)).  Numbers without rows have no steps.
-    __device__ static __forceinline__ int number(int G, int s, int cu) { return (int)((int64_t)cu * G / R) + s; }
+    __device__ static __forceinline__ int number(int G, int s, int cu) { return paged_number<R>(G, s, cu); }
     __device__ static __forceinline__ int cu(const PagedAttn& a, const PWalkLds& m, int s) { return a.t.S <= PWalkLds::MAX ? m.cu[s] : a.t.cu_q[s]; }
 
     // tile t of slot s, which is moved on to the one whose numbers t is among: its rows, its key steps (0: a number without rows; a tile that sees no key takes one, fully masked).
@@ -669,17 +672,16 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_keys_k(
     int part = 0, parts = 0, per = 0;
     w.g = id % a.Hkv;
     const bool work = paged_unit(a, id / a.Hkv, w, part, parts, per);
-    if (a.target && tid == 0) {
-        if (id == 0) paged_cut(a)->used = gridDim.x;
-        PCut* c = paged_cut(a) + id;
+    if (!work) return;
+    if (a.target && tid == 0 && part == 0) {                                           // the item's record is at its number
+        PCut* c = paged_cut(a) + (int64_t)(paged_number<32>(a.G, w.s, w.q0) + (w.row0 >> 5)) * a.Hkv + w.g;
         c->first = id;
-        c->parts = work && part == 0 ? parts : 0;
+        c->parts = parts;
         c->q0 = w.q0;
         c->row0 = w.row0;
         c->rows = w.rows;
         c->g = w.g;
     }
-    if (!work) return;
     const int kmax = min(paged_seen(a, w.len, w.n, (min(w.row0 + 32, w.rows) - 1) / a.G), w.len), k0 = part * per << a.sh;
     const int t0 = k0 >> 5, t1 = min((kmax + 31) >> 5, part + 1 == parts ? 0x7fffffff : (k0 + (per << a.sh)) >> 5);       // 32-key steps
     char* kb = smem + wave * STAGE;
@@ -770,6 +772,17 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_keys_k(
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
+// Does tile number t of 32 rows exist, that is, was its record written?  (a slot a lane)
+__device__ __forceinline__ bool paged_tile_exists(const PagedAttn& a, int t) {
+    const int lane = threadIdx.x & 63;
+    bool is = false;
+    for (int s0 = 0; s0 < a.t.S; s0 += 64) {
+        const int s = min(s0 + lane, a.t.S - 1), c0 = a.t.cu_q[s], c1 = a.t.cu_q[s + 1], row0 = (t - paged_number<32>(a.G, s, c0)) * 32;
+        is |= s0 + lane < a.t.S && c0 >= 0 && c1 > c0 && c1 <= a.N && row0 >= 0 && row0 < (c1 - c0) * a.G;
+    }
+    return __any(is);
+}
+
 // The join of cut items.  blockIdx.x: the item's record.  A thread adds one quad of dims of one row over the parts, in their order, with weights 2^(m_p - m); eight lanes
 // read 128 bytes of a part as the lanes of the tile kernel left them.  PG = 4 (few rows, many parts: the keys kernel): each wave takes a quarter of the parts, they meet in LDS.
 // ---------------------------------------------------------------------------------------------------------------------------------
@@ -777,8 +790,8 @@ template <int HDP, int R, int PG>
 __global__ __launch_bounds__(256) void attn_paged_join_k(PagedAttn a) {
     constexpr int T = 256 / PG, U = PG > 1 ? 8 : 4;                                    // threads over (row, quad); parts in flight
     __shared__ float red[PG > 1 ? PG - 1 : 1][6][64];
-    if ((int)blockIdx.x >= paged_cut(a)->used) return;
     const PCut c = paged_cut(a)[blockIdx.x];
+    if (PG > 1 ? !paged_tile_exists(a, blockIdx.x / a.Hkv) : (int)blockIdx.x >= paged_cut(a)->used) return;
     const int step = PG > 1 ? a.Hkv : 1;                                                // keys kernel: the units of a head; tile kernel: the workers, two parts each
     if (c.parts < 2 || c.first < 0 || c.first + (c.parts - 1) * step >= a.blocks) return;
     const int pg = PG > 1 ? threadIdx.x / T : 0, per = (c.parts + PG - 1) / PG, pb = min(pg * per, c.parts), pe = min(pb + per, c.parts);
@@ -896,7 +909,7 @@ int launch(const PagedAttn& a, const Plan& p, hipStream_t st) {
         constexpr int NW = 4, smem = NW * 64 * PCfg<HDP>::P;
         UFV_ONCE_PER_DEVICE((void)hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_keys_k<HDP, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, smem););
         hipLaunchKernelGGL((attn_paged_keys_k<HDP, NW>), dim3(a.blocks), dim3(NW * 64), smem, st, a);
-        if (p.target) hipLaunchKernelGGL((attn_paged_join_k<HDP, 32, 4>), dim3(a.blocks, HDP / 32), dim3(256), 0, st, a);
+        if (p.target) hipLaunchKernelGGL((attn_paged_join_k<HDP, 32, 4>), dim3(a.tiles * a.Hkv, HDP / 32), dim3(256), 0, st, a);
     } else if (p.rows == 256) {
         if constexpr (HDP > 64 && HDP <= 128) launch_tile<HDP, 8, 4>(a, st);
     } else {
