@@ -282,14 +282,6 @@ __global__ __launch_bounds__(1024) void kv_pages_plan_k(int* refs, int n_pages, 
     if (tid == 0) { counts[0] = live; counts[1] = movers; }
 }
 
-__global__ __launch_bounds__(256) void kv_pages_remap_k(int* table, int64_t ld, int width, const int* __restrict__ kv_len, const int* __restrict__ remap, int n_pages, int sh) {
-    const int s = blockIdx.x, n = pages_held(kv_len[s], sh, width);
-    for (int j = threadIdx.x; j < n; j += 256) {
-        const int id = table[(int64_t)s * ld + j];
-        if ((unsigned)id < (unsigned)n_pages) table[(int64_t)s * ld + j] = remap[id];
-    }
-}
-
 // 16 KB of one page: 256 threads x 4 x 16 bytes, all four loads before the first store
 __device__ __forceinline__ void copy_piece(const char* __restrict__ src, char* __restrict__ dst, int64_t bytes, int64_t at) {
     typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
@@ -317,8 +309,17 @@ __global__ __launch_bounds__(256) void kv_pages_copy_k(char* pool, int64_t layer
     copy_piece(base + src * page_bytes, base + dst * page_bytes, bytes, at);
 }
 
-// the moves of kv_pages_plan_k (their number is known on the device only): a fixed grid walks over (move, layer, 16 KB piece)
-__global__ __launch_bounds__(256) void kv_pages_move_k(char* pool, int layers, int64_t layer_bytes, int64_t page_bytes, int n_pages, const int* __restrict__ counts, const int* __restrict__ ws) {
+// the moves of kv_pages_plan_k (their number is known on the device only): a fixed grid walks over (move, layer, 16 KB piece).  The first blocks rewrite the table rows before that: a launch
+// of its own for them cost 2.6 us.
+__global__ __launch_bounds__(256) void kv_pages_move_k(char* pool, int layers, int64_t layer_bytes, int64_t page_bytes, int n_pages, const int* __restrict__ counts, const int* __restrict__ ws,
+                                                       int* table, int64_t ld, int width, const int* __restrict__ kv_len, int S, int sh) {
+    for (int s = blockIdx.x; s < S; s += gridDim.x) {
+        const int n = pages_held(kv_len[s], sh, width);
+        for (int j = threadIdx.x; j < n; j += 256) {
+            const int id = table[(int64_t)s * ld + j];
+            if ((unsigned)id < (unsigned)n_pages) table[(int64_t)s * ld + j] = ws[2 * (int64_t)n_pages + id];
+        }
+    }
     const int pieces = (int)((page_bytes + 16383) / 16384);
     const int64_t total = (int64_t)counts[1] * layers * pieces;
     for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
@@ -433,8 +434,8 @@ extern "C" int ufv_kv_pages_compact(void* pool, int layers, int64_t layer_bytes,
                 (long long)ufv_kv_pages_compact_ws_bytes(n_pages));
     const int sh = paged_log2(page);
     hipLaunchKernelGGL(kv_pages_plan_k, dim3(1), dim3(1024), 0, ST(stream), refs, n_pages, counts, (int*)ws);
-    hipLaunchKernelGGL(kv_pages_remap_k, dim3(S), dim3(256), 0, ST(stream), block_table, ld_table, max_pages, kv_len, (const int*)ws + 2 * (int64_t)n_pages, n_pages, sh);
-    hipLaunchKernelGGL(kv_pages_move_k, dim3(2048), dim3(256), 0, ST(stream), (char*)pool, layers, layer_bytes, page * row_bytes, n_pages, counts, (const int*)ws);
+    hipLaunchKernelGGL(kv_pages_move_k, dim3(2048), dim3(256), 0, ST(stream), (char*)pool, layers, layer_bytes, page * row_bytes, n_pages, counts, (const int*)ws,
+                       block_table, ld_table, max_pages, kv_len, S, sh);
     UFV_CHECK_LAUNCH();
     return UFV_OK;
 }
