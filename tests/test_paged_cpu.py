@@ -66,6 +66,29 @@ def test_paged_entry_points_refuse_bad_arguments():
         _refused("ufv_kv_pages_compact", co, **bad)
 
 
+def test_attention_paged_refuses_what_its_kernels_do_not_hold_for():
+    keep, p = _buf()
+    att = dict(q=p, ldq=3584, o=p, ldo=3584, N=3, Hq=28, Hkv=4, hd=128, pages=p, n_pages=4, page=64, ldkv=1024, table=p, ld_table=2, max_pages=2, cu=p, kl=p, S=2, scale=0.1, causal=1, ws=p,
+               ws_bytes=1 << 40, stream=0)
+    for bad in (dict(scale=0.0), dict(scale=-0.1), dict(scale=float("inf")), dict(scale=float("nan")), dict(ldkv=1 << 24), dict(hd=264), dict(S=1 << 24), dict(N=1 << 27)):
+        _refused("ufv_attention_paged", att, **bad)
+    lib = _lib.load()
+    for N, S, max_pages in ((2, 2, 64), (300, 2, 64), (4000, 2, 64)):
+        need = lib.ufv_attention_paged_ws_bytes(N, S, 28, 4, 128, max_pages * 64)
+        assert need > 0
+        for bad in (dict(ws_bytes=need - 1), dict(ws=0), dict(ws=p + 8)):
+            _refused("ufv_attention_paged", dict(att, N=N, S=S, max_pages=max_pages, ld_table=max_pages), **bad)
+
+
+def test_attention_paged_workspace_does_not_grow_with_the_cache():
+    """parts are a number of the card, not of the lengths or the slots; what grows with the slots is one record for each item"""
+    ws = _lib.load().ufv_attention_paged_ws_bytes
+    assert ws(1, 1, 28, 4, 128, 512) == 0
+    one = ws(1, 1, 28, 4, 128, 1 << 20)
+    assert one == ws(1, 1, 28, 4, 128, 1 << 24) and ws(5000, 5000, 28, 4, 128, 1 << 20) < 2 * one
+    assert ws(16383, 1, 28, 4, 128, 1 << 24) == ws(16383, 1, 28, 4, 128, 1 << 20)
+
+
 def test_paged_ops_refuse_tensors_off_the_gpu_and_wrong_shapes():
     bf, i32 = torch.bfloat16, torch.int32
     pages = torch.zeros(4, 16, 128, dtype=bf)

@@ -546,3 +546,52 @@ def test_attention_paged_many_short_items(q, kv, Hq, Hkv, hd):
     """items of one to four steps, so many that the ends of the blocks' shares fall close behind, into and close before short items"""
     n = 300
     run_case([max(q - (i * 7) % 5, 1) for i in range(n)], [kv + (i * 11) % 70 for i in range(n)], Hq, Hkv, hd, 16, seed=q)
+
+
+@pytest.mark.parametrize("q,kv,Hq,Hkv,hd", [(300, 2400, 8, 1, 96), (280, 2100, 16, 2, 104), (2100, 2100, 3, 3, 72), (300, 2111, 28, 4, 128), (700, 2050, 12, 4, 128)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_paged_wide_tiles(q, kv, Hq, Hkv, hd, causal):
+    """slots of 2048 rows and more over 2048 keys and more"""
+    run_case([q], [kv], Hq, Hkv, hd, 64, causal=causal, seed=q)
+
+
+@pytest.mark.parametrize("q", [1, 40])
+def test_attention_paged_hundreds_of_slots(q):
+    """more slots than fit the copy of their lengths on chip; every ninth has no new token"""
+    n = 700
+    run_case([0 if i % 9 == 4 else q for i in range(n)], [q + (i * 37) % 150 for i in range(n)], 4, 4, 16, 16, seed=q)
+
+
+@pytest.mark.parametrize("q,kv,Hq,Hkv,hd,lo,hi", [(1, 9000, 28, 4, 128, 1000, 3000), (1, 9000, 4, 4, 64, 8000, 9000), (300, 4000, 28, 4, 128, 0, 2000), (100, 6000, 4, 2, 64, 2000, 5000)])
+def test_attention_paged_stretch_of_nan_reaches_every_row(q, kv, Hq, Hkv, hd, lo, hi):
+    """K rows of NaN, more of them than a block's keys: a part with no number in it leaves NaN, not nothing"""
+    b = Batch([q, 1], [kv, 50], Hkv, hd, 64, device=DEV)
+    for j in range(lo, hi):
+        b.pages[b.row(0, j)] = float("nan")
+    out = ops.attention_paged(rnd(q + 1, Hq * hd).to(BF), b.pages, b.table, b.cu_q, b.kv_len, Hq, Hkv, hd)
+    assert torch.isnan(out[:q]).all() and torch.isfinite(out[q:]).all()
+
+
+def test_attention_paged_nan_in_a_new_key_stays_with_the_rows_that_see_it():
+    for q, kv, at in ((300, 4000, 3900), (20, 3000, 2990)):
+        b = Batch([q], [kv], 4, 128, 64, device=DEV)
+        b.pages[b.row(0, at)] = float("nan")
+        out = ops.attention_paged(rnd(q, 28 * 128).to(BF), b.pages, b.table, b.cu_q, b.kv_len, 28, 4, 128)
+        first = at - (kv - q)
+        assert torch.isfinite(out[:first]).all() and torch.isnan(out[first:]).all()
+
+
+def test_attention_paged_new_workspace_contents_do_not_show():
+    """the workspace is not cleared between calls: whatever it holds, results are the same bit for bit"""
+    for q, kv, Hq, Hkv, hd in (([1, 1, 0, 1], [9000, 40, 7, 700], 28, 4, 128), ([300, 5], [4000, 900], 28, 4, 128), ([70, 64], [300, 1000], 14, 2, 64)):
+        b = Batch(q, kv, Hkv, hd, 64, device=DEV)
+        x, outs = rnd(b.N, Hq * hd).to(BF), []
+        n = ops._attention_paged_ws(b.N, len(q), Hq, Hkv, hd, b.table.shape[1] * 64)
+        for fill in (0, 1, 255, 127):
+            w = torch.full((max(n, 16),), fill, device=DEV, dtype=torch.uint8)
+            out = torch.zeros(b.N, Hq * hd, device=DEV, dtype=BF)
+            _lib.call("ufv_attention_paged", x.data_ptr(), Hq * hd, out.data_ptr(), Hq * hd, b.N, Hq, Hkv, hd, b.pages.data_ptr(), b.P, 64, 2 * Hkv * hd, b.table.data_ptr(), b.table.shape[1],
+                      b.table.shape[1], b.cu_q.data_ptr(), b.kv_len.data_ptr(), len(q), hd ** -0.5, 1, w.data_ptr(), n, torch.cuda.current_stream().cuda_stream)
+            torch.cuda.synchronize()
+            outs.append(out)
+        assert all(torch.equal(outs[0], o) for o in outs) and outs[0].abs().max() > 0

@@ -25,21 +25,22 @@ struct PagedAttn {
     PagedTable t;
     int N, Hq, Hkv, G, hd, causal;
     float sl2;              // scale * log2(e)
-    int tiles, blocks;      // row tiles (upper bound), records and workers
+    int tiles;              // row tiles (upper bound)
     int target, sh;         // keys kernel: parts of a head that are aimed at (0: no item is cut), log2 of the keys of its step
-    float* part;            // PCut [blocks], parts (paged_part)
+    int cuts, parts;        // what the workspace holds: PCut [cuts], then the parts (paged_part)
+    float* ws;
 };
 
 // What the join has to know of an item that several blocks worked on (parts = 0: nothing to do).  A part is un-normalised O as the lanes of the tile kernel hold it --
 // [32 rows][HDP / 8][64 lanes][4], so that every store is whole lines -- then R pairs (max, sum).
-struct PCut { int first, parts;               // its first part's block; the number of its parts
+struct PCut { int first, parts;               // its first part (tile kernel: that part's worker); the number of its parts
               int q0, row0, rows, g;          // as in PagedTile
               int used, pad; };               // (of the first: how many records are valid)
-__device__ __forceinline__ PCut* paged_cut(const PagedAttn& a) { return reinterpret_cast<PCut*>(a.part); }
+__device__ __forceinline__ PCut* paged_cut(const PagedAttn& a) { return reinterpret_cast<PCut*>(a.ws); }
 template <int HDP>
 __device__ __forceinline__ int part_at(int row, int quad) { return (((row >> 5) * (HDP / 8) + (quad >> 1)) * 64 + (quad & 1) * 32 + (row & 31)) * 4; }
 template <int HDP, int R>
-__device__ __forceinline__ float* paged_part(const PagedAttn& a, int i) { return a.part + (int64_t)a.blocks * (sizeof(PCut) / 4) + (int64_t)i * (R * (HDP + 2)); }
+__device__ __forceinline__ float* paged_part(const PagedAttn& a, int i) { return a.ws + (int64_t)a.cuts * (sizeof(PCut) / 4) + (int64_t)i * (R * (HDP + 2)); }
 
 // what a block works on: all of it wave-uniform
 struct PagedTile {
@@ -55,6 +56,26 @@ __device__ __forceinline__ int paged_number(int G, int s, int cu) { return (int)
 
 // keys that row r of a slot sees: tokens 0 .. paged_seen - 1
 __device__ __forceinline__ int paged_seen(const PagedAttn& a, int len, int n, int tok) { return a.causal ? max(len - n + tok + 1, 0) : len; }
+
+// inclusive prefix sums over the wave, by lane shifts within rows of 16 and the row ends passed on
+template <int CTRL, int ROWS, class T>
+__device__ __forceinline__ T lane_shift(T x) {
+    if constexpr (sizeof(T) == 8) {
+        const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, ROWS, 0xf, false);
+        return (T)((uint64_t)hi << 32 | lo);
+    } else {
+        return (T)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+    }
+}
+template <class T>
+__device__ __forceinline__ T lane_scan(T x) {
+    x += lane_shift<0x111, 0xf>(x);                       // row_shr 1, 2, 4, 8
+    x += lane_shift<0x112, 0xf>(x);
+    x += lane_shift<0x114, 0xf>(x);
+    x += lane_shift<0x118, 0xf>(x);
+    x += lane_shift<0x142, 0xa>(x);                       // row_bcast 15 into rows 1 and 3, 31 into rows 2 and 3
+    return x + lane_shift<0x143, 0xc>(x);
+}
 
 __device__ __forceinline__ bf16x8 pack8(const float* p) {
     bf16x8 r;
@@ -385,12 +406,7 @@ struct PWalk {
         int64_t mine = 0;
         int s1 = s;
         for (int t = t0; t < t1; ++t) mine += steps(t, s1);
-        int64_t x = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int64_t y = __shfl_up((long long)x, o, 64);
-            if (lane >= o) x += y;
-        }
+        const int64_t x = lane_scan(mine);
         if (lane == 63) m.scan[wave] = x;
         __syncthreads();
         int64_t before = x - mine;
@@ -612,7 +628,7 @@ constexpr int STEP_SH = 7;                 // log2 of the keys of a step: 4 wave
 
 // What unit u of a head is: its tile, its keys [k0, k1) in steps, part of parts.  Every wave finds it for itself, a slot a lane, with one round of loads: sums the steps of the batch for the
 // length of a part, then the slots' units.
-__device__ __forceinline__ bool paged_unit(const PagedAttn& a, int u, PagedTile& w, int& part, int& parts, int& per) {
+__device__ __forceinline__ bool paged_unit(const PagedAttn& a, int u, PagedTile& w, int& part, int& parts, int& per, int& first) {
     const int lane = threadIdx.x & 63;
     int c0, n, len, tiles, steps;
     auto load = [&](int s0) {
@@ -629,21 +645,18 @@ __device__ __forceinline__ bool paged_unit(const PagedAttn& a, int u, PagedTile&
         load(s0);
         all += (unsigned)tiles * (unsigned)steps;                                      // (below 2^31 over the batch: see `sh`)
     }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) all += __shfl_xor(all, o, 64);
+    all = __builtin_amdgcn_readlane(lane_scan(all), 63);
     const int length = a.target ? max((int)((all + a.target - 1) / a.target), 1) : 1 << 30;
-    int before = 0;
+    int before = 0, cut = 0;                                                           // units, units of cut items of the slots before
     for (int s0 = 0; s0 < a.t.S; s0 += 64) {
         if (a.t.S > 64) load(s0);
-        const int most = max((steps + length - 1) / length, 1), p = max((steps + most - 1) / most, 1), k = max((steps + p - 1) / p, 1), mine = tiles * k;
-        int x = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int y = __shfl_up(x, o, 64);
-            if (lane >= o) x += y;
+        const int most = max((steps + length - 1) / length, 1), p = max((steps + most - 1) / most, 1), k = max((steps + p - 1) / p, 1), mine = tiles * k, mc = k > 1 ? mine : 0;
+        const int x = lane_scan(mine), xc = lane_scan(mc), c = __popcll(__ballot(before + x <= u));
+        if (c == 64) {
+            before += __builtin_amdgcn_readlane(x, 63);
+            cut += __builtin_amdgcn_readlane(xc, 63);
+            continue;
         }
-        const int c = __popcll(__ballot(before + x <= u));
-        if (c == 64) { before += __builtin_amdgcn_readlane(x, 63); continue; }
         parts = __builtin_amdgcn_readlane(k, c);
         per = __builtin_amdgcn_readlane(p, c);
         w.s = s0 + c;
@@ -652,9 +665,11 @@ __device__ __forceinline__ bool paged_unit(const PagedAttn& a, int u, PagedTile&
         w.len = __builtin_amdgcn_readlane(len, c);
         w.rows = w.n * a.G;
         const int r = u - before - __builtin_amdgcn_readlane(x - mine, c);
+        if (r < 0) return false;                                                       // (cu_q that does not ascend: nothing outside the arrays is touched)
         w.row0 = r / parts * 32;
         part = r % parts;
-        return true;
+        first = cut + __builtin_amdgcn_readlane(xc - mc, c) + r - part;
+        return w.row0 < w.rows && (parts == 1 || (first >= 0 && (int64_t)(first + parts) * a.Hkv <= a.parts));
     }
     return false;
 }
@@ -669,13 +684,13 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_keys_k(
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = lane >> 5, l31 = lane & 31, id = blockIdx.x;
     PagedTile w = {};
-    int part = 0, parts = 0, per = 0;
+    int part = 0, parts = 0, per = 0, first = 0;
     w.g = id % a.Hkv;
-    const bool work = paged_unit(a, id / a.Hkv, w, part, parts, per);
+    const bool work = paged_unit(a, id / a.Hkv, w, part, parts, per, first);
     if (!work) return;
     if (a.target && tid == 0 && part == 0) {                                           // the item's record is at its number
         PCut* c = paged_cut(a) + (int64_t)(paged_number<32>(a.G, w.s, w.q0) + (w.row0 >> 5)) * a.Hkv + w.g;
-        c->first = id;
+        c->first = first * a.Hkv + w.g;
         c->parts = parts;
         c->q0 = w.q0;
         c->row0 = w.row0;
@@ -764,7 +779,7 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_keys_k(
             const float inv = sum > 0.f ? 1.f / sum : sum;
             *reinterpret_cast<bf16x4*>(a.o + (int64_t)(w.q0 + tok) * a.ldo + hq * a.hd + quad * 4) = bf16x4{(bf16)(o[0] * inv), (bf16)(o[1] * inv), (bf16)(o[2] * inv), (bf16)(o[3] * inv)};
         } else {
-            float* dst = paged_part<HDP, 32>(a, id);
+            float* dst = paged_part<HDP, 32>(a, (first + part) * a.Hkv + w.g);
             *reinterpret_cast<f32x4*>(dst + part_at<HDP>(r, quad)) = o;
             if (quad == 0) *reinterpret_cast<f32x2*>(dst + 32 * HDP + 2 * r) = f32x2{m, sum};
         }
@@ -792,8 +807,9 @@ __global__ __launch_bounds__(256) void attn_paged_join_k(PagedAttn a) {
     __shared__ float red[PG > 1 ? PG - 1 : 1][6][64];
     const PCut c = paged_cut(a)[blockIdx.x];
     if (PG > 1 ? !paged_tile_exists(a, blockIdx.x / a.Hkv) : (int)blockIdx.x >= paged_cut(a)->used) return;
-    const int step = PG > 1 ? a.Hkv : 1;                                                // keys kernel: the units of a head; tile kernel: the workers, two parts each
-    if (c.parts < 2 || c.first < 0 || c.first + (c.parts - 1) * step >= a.blocks) return;
+    const int step = PG > 1 ? a.Hkv : 1;                                                // keys kernel: the parts of a head; tile kernel: the workers, two parts each
+    if (c.parts < 2 || c.first < 0 || c.first + (int64_t)(c.parts - 1) * step >= (PG > 1 ? a.parts : a.cuts)) return;
+    if (c.q0 < 0 || c.row0 < 0 || c.rows > (int64_t)(a.N - c.q0) * a.G || (unsigned)c.g >= (unsigned)a.Hkv) return;   // (a record that nobody wrote: cu_q that does not ascend)
     const int pg = PG > 1 ? threadIdx.x / T : 0, per = (c.parts + PG - 1) / PG, pb = min(pg * per, c.parts), pe = min(pb + per, c.parts);
     for (int i0 = blockIdx.y * T; i0 < R * (HDP / 4); i0 += gridDim.y * T) {
         const int i = i0 + threadIdx.x % T, quad = (i >> 3) % (HDP / 4), row = (i >> 3) / (HDP / 4) * 8 + (i & 7), r = c.row0 + row;
@@ -864,7 +880,8 @@ __global__ __launch_bounds__(256) void attn_paged_join_k(PagedAttn a) {
 struct Plan {
     bool keys;              // keys split over the waves (else rows)
     int rows, tiles;        // of a tile; upper bound of their number
-    int blocks, target, sh; // as in PagedAttn
+    int blocks;             // of the kernel
+    int target, sh, cuts, parts;               // as in PagedAttn
     int64_t ws;             // bytes
 };
 
@@ -884,23 +901,26 @@ Plan make_plan(int N, int S, int Hq, int Hkv, int hd, int max_keys) {
         p.target = max_keys > 4 << STEP_SH ? (TARGET + Hkv - 1) / Hkv : 0;                // (333 tokens in one block 10.3 us, in three and joined 10.2)
         p.blocks = (p.target + p.tiles) * Hkv;
         for (p.sh = STEP_SH; (int64_t)p.tiles * ((max_keys >> p.sh) + 1) > 0x7fffffff;) ++p.sh;
-        p.ws = p.target ? (int64_t)p.blocks * ((int64_t)sizeof(PCut) + 4 * 32 * (hdp + 2)) : 0;
+        p.cuts = p.target ? p.tiles * Hkv : 0;
+        p.parts = 2 * p.target * Hkv;          // an item that is cut is longer than a part: its parts are at most twice its length in parts
     } else {
         // what fits the CUs at once: three blocks of four waves up to head_dim 64, two up to 128, one above; one block of eight
         const int slots = hd > 128 || p.rows == 256 ? 256 : (hd <= 64 ? 768 : 512);
         const int64_t steps = (rows / p.rows + used) * Hkv * (((int64_t)max_keys + 63) / 64 + ITEM_COST);
         p.blocks = steps / MIN_SHARE >= slots ? slots : (int)((steps / MIN_SHARE + 8) / 8 * 8);
-        p.ws = (int64_t)p.blocks * ((int64_t)sizeof(PCut) + 2 * 4 * p.rows * (hdp + 2));
+        p.cuts = p.blocks;
+        p.parts = 2 * p.blocks;
     }
+    p.ws = (int64_t)p.cuts * (int64_t)sizeof(PCut) + (int64_t)p.parts * 4 * p.rows * (hdp + 2);
     return p;
 }
 
 template <int HDP, int NW, int NS>
-void launch_tile(const PagedAttn& a, hipStream_t st) {
+void launch_tile(const PagedAttn& a, int blocks, hipStream_t st) {
     constexpr int smem = NS * 128 * PCfg<HDP>::P;
     UFV_ONCE_PER_DEVICE((void)hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_tile_k<HDP, NW, NS>), hipFuncAttributeMaxDynamicSharedMemorySize, smem););
-    hipLaunchKernelGGL((attn_paged_tile_k<HDP, NW, NS>), dim3(a.blocks), dim3(NW * 64), smem, st, a);
-    hipLaunchKernelGGL((attn_paged_join_k<HDP, 32 * NW, 1>), dim3(a.blocks, 32 * NW * (HDP / 4) / 256), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_paged_tile_k<HDP, NW, NS>), dim3(blocks), dim3(NW * 64), smem, st, a);
+    hipLaunchKernelGGL((attn_paged_join_k<HDP, 32 * NW, 1>), dim3(blocks, 32 * NW * (HDP / 4) / 256), dim3(256), 0, st, a);
 }
 
 template <int HDP>
@@ -908,12 +928,12 @@ int launch(const PagedAttn& a, const Plan& p, hipStream_t st) {
     if (p.keys) {
         constexpr int NW = 4, smem = NW * 64 * PCfg<HDP>::P;
         UFV_ONCE_PER_DEVICE((void)hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_keys_k<HDP, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, smem););
-        hipLaunchKernelGGL((attn_paged_keys_k<HDP, NW>), dim3(a.blocks), dim3(NW * 64), smem, st, a);
+        hipLaunchKernelGGL((attn_paged_keys_k<HDP, NW>), dim3(p.blocks), dim3(NW * 64), smem, st, a);
         if (p.target) hipLaunchKernelGGL((attn_paged_join_k<HDP, 32, 4>), dim3(a.tiles * a.Hkv, HDP / 32), dim3(256), 0, st, a);
     } else if (p.rows == 256) {
-        if constexpr (HDP > 64 && HDP <= 128) launch_tile<HDP, 8, 4>(a, st);
+        if constexpr (HDP > 64 && HDP <= 128) launch_tile<HDP, 8, 4>(a, p.blocks, st);
     } else {
-        launch_tile<HDP, 4, (HDP <= 64 ? 3 : 2)>(a, st);
+        launch_tile<HDP, 4, (HDP <= 64 ? 3 : 2)>(a, p.blocks, st);
     }
     UFV_CHECK_LAUNCH();
     return UFV_OK;
@@ -938,7 +958,7 @@ extern "C" int ufv_attention_paged(const void* q, int64_t ldq, void* o, int64_t 
     UFV_REQUIRE(ldkv >= 2 * (int64_t)Hkv * hd && ldkv < 1 << 24 && (N == 1 || (ldq >= (int64_t)Hq * hd && ldo >= (int64_t)Hq * hd)), "ufv_attention_paged: a row pitch is out of range");
     UFV_REQUIRE((int64_t)N * Hq < 0x7fffffff && S < 1 << 24, "ufv_attention_paged: too many rows or slots (N=%d S=%d)", N, S);
     const Plan p = make_plan(N, S, Hq, Hkv, hd, max_pages << paged_log2(page));
-    UFV_REQUIRE(((int64_t)p.tiles + p.target) * Hkv < 0x7fffffff && Hkv < 65536, "ufv_attention_paged: too many row tiles (N=%d S=%d)", N, S);
+    UFV_REQUIRE(((int64_t)p.tiles + 2 * p.target) * Hkv < 0x7fffffff && Hkv < 65536, "ufv_attention_paged: too many row tiles (N=%d S=%d)", N, S);
     UFV_REQUIRE(p.ws == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= p.ws), "ufv_attention_paged: a 16-byte aligned workspace of %lld bytes is needed (%lld given)", (long long)p.ws,
                 (long long)ws_bytes);
     PagedAttn a;
@@ -947,7 +967,7 @@ extern "C" int ufv_attention_paged(const void* q, int64_t ldq, void* o, int64_t 
     a.t = PagedTable{block_table, ld_table, max_pages, cu_q, kv_len, S, n_pages, paged_log2(page)};
     a.N = N; a.Hq = Hq; a.Hkv = Hkv; a.G = Hq / Hkv; a.hd = hd; a.causal = causal != 0;
     a.sl2 = scale * 1.4426950408889634f;
-    a.tiles = p.tiles; a.blocks = p.blocks; a.target = p.target; a.sh = p.sh; a.part = (float*)ws;
+    a.tiles = p.tiles; a.target = p.target; a.sh = p.sh; a.cuts = p.cuts; a.parts = p.parts; a.ws = (float*)ws;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (hd <= 32) return launch<32>(a, p, st);
     if (hd <= 64) return launch<64>(a, p, st);
