@@ -8,9 +8,11 @@
 // Both kernels compute S^T = K Q^T with v_mfma_f32_32x32x16_bf16 (a lane owns one row of the tile: its column of S^T), keep the running maximum and sum of the softmax in
 // 32 bits (log2 domain), and use the exponentiated tile, rounded to bf16, directly as the B operand of O^T += V^T P^T.  The rounding of P is the one step below 32 bits between
 // the inputs and the output: the matrix instruction takes bf16 operands; the row sum is taken of the unrounded values.  V^T fragments come from row-major V rows in LDS by the transposing read.
-//   attn_paged_tile_k   the waves of a block share 64-key tiles and split the ROWS: chunks of many rows, bound by the matrix unit
-//   attn_paged_keys_k   the waves of a block share up to 32 rows and split the KEYS: a few new tokens over a long cache, bound by the bytes of the cache
-// Either may be split further over the keys by blocks (few tiles on 256 CUs); the parts leave (max, sum, un-normalised O) in 32 bits in the workspace and attn_paged_join_k adds them in order.
+//   attn_paged_tile_k   the waves of a block share 64-key tiles and split the ROWS: chunks of many rows, bound by the matrix unit.  28 / 4 heads of 128: 2399 tokens over 20011 in 660 us
+//                       (0.98 PF/s with its join), 8192 causal tokens 600 us, 16 questions of 9 .. 83 tokens behind 2304 shared ones 58 us (0.43 PF/s: 13 steps a block, then the join)
+//   attn_paged_keys_k   the waves of a block share up to 32 rows and split the KEYS: a few new tokens over a long cache, bound by the bytes of the cache.  48 slots of 714 .. 5825 tokens
+//                       57 us (5.0 TB/s; a large read reaches 6.1), one of 31999 24 us (2.8 TB/s: 4 us until the first keys are asked for, 5 us for the join)
+// The work is cut over the keys for the 256 CUs; the parts leave (max, sum, un-normalised O) in 32 bits in the workspace and attn_paged_join_k adds them in order.
 #include "paged.h"
 
 namespace {
@@ -125,8 +127,12 @@ struct PState {
 // NH half tiles of 32 keys in LDS (K rows at kb, V rows at vb) against 32 rows: S^T, running softmax, O^T.  hide: key j of the step counts for the lane's row iff j < vis and, in groups of 16
 // keys, iff its bit of `groups` is set.
 // at_qk(i, n, next) runs behind the i-th of the n products of S^T: the loads of a later step (memory -> LDS at `next`) go there, a few at a time -- issued in one go they hold the wave for
-// 1300 of the 4900 cycles of a step (the memory pipe takes one 1 KB load in 16 cycles), behind the products they cost little.  kb, vb, next do not overlap (__restrict__ lets the compiler
+// 1300 of the 4500 cycles of a step (the memory pipe takes one 1 KB load in 16 cycles), behind the products they cost little.  kb, vb, next do not overlap (__restrict__ lets the compiler
 // keep the loads in flight across the reads: who issues them waits for them before the barrier that publishes them).
+// A step of 64 keys at head_dim 128 is 1024 cycles of the matrix unit, two waves a SIMD: 2048.  16384 rows over 8192 keys run at 1.05 PF/s (4400 cycles a step); without the LDS reads they would
+// take 5 % less, without the exponentials 7 %, without the loads 7 %, without all three 21 % -- no one of them bounds it, and then the clock falls: the products alone reach 1.26 PF/s, a large
+// library product 1.42.  Tried and slower: the exponentials between the products of the next step's S^T (8 %; the maximum between those of O^T), 64 rows a wave (30 %), waves in two groups
+// half a step apart (4 %).
 template <int HDP, int NH, class FQ>
 __device__ __forceinline__ void paged_step(const char* __restrict__ kb, const char* __restrict__ vb, char* __restrict__ next, const bf16x8 (&qf)[HDP / 16], PState<HDP>& st, float sl2, bool hide, int vis,
                                            unsigned groups, FQ&& at_qk) {
@@ -487,7 +493,7 @@ struct PWalk {
 };
 
 template <int HDP, int NW, int NS>
-__global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_tile_k(PagedAttn a) {
+__global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : HDP > 32 ? 2 : 4) void attn_paged_tile_k(PagedAttn a) {
     using C = PCfg<HDP>;
     constexpr int R = 32 * NW, HALF = 64 * C::P, STAGE = 2 * HALF;                         // a step's K rows, its K and V rows
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -506,7 +512,7 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_tile_k(
     F fe;
     PState<HDP> st;
     bf16x8 qf[C::KS];
-    PagedTile w = {}, old = {};                                                                  // the item, the one before
+    PagedTile w = {}, old = {};                                                        // the item, the one before
     int t0 = 0, t1 = 0, seen = 0, seen_min = 0, diag = 0;
     bool cut = false;                                                                  // the item lies in several shares
     int ids = 0, ids2 = 0;                                                             // of the step to be fetched next and its neighbours, of the chunk behind it
@@ -891,7 +897,7 @@ Plan make_plan(int N, int S, int Hq, int Hkv, int hd, int max_keys) {
     const int64_t rows = (int64_t)N * G;
     Plan p = {};
     p.keys = rows <= 32 * (int64_t)S;
-    // Tiles of 256 rows (eight waves, one block a CU, a ring of four steps) fetch a key once for 256 rows, those of 128 (two or three blocks a CU, a ring of two or three) waste fewer rows and
+    // Tiles of 256 rows (eight waves, one block a CU, a ring of four steps) fetch a key once for 256 rows, those of 128 (two to four blocks a CU, a ring of two) waste fewer rows and
     // steps on short slots and sequences.  28 / 4 heads of 128, 128 | 256: 2399 tokens over 20011 757 | 679 us, 8192 causal 675 | 606, 8 x 512 over 4096 289 | 261, 16 x 150 over 2048
     // 117 | 120, 4 x 100 over 2048 38 | 39, 8 x 600 causal 69 | 76, 300 causal 22 | 27; 14 / 2 heads of 64: 8192 tokens 412 | 443, 4 x 300 22 | 33.  Above 128 the registers of 256 rows do
     // not fit.
@@ -904,8 +910,9 @@ Plan make_plan(int N, int S, int Hq, int Hkv, int hd, int max_keys) {
         p.cuts = p.target ? p.tiles * Hkv : 0;
         p.parts = 2 * p.target * Hkv;          // an item that is cut is longer than a part: its parts are at most twice its length in parts
     } else {
-        // what fits the CUs at once: three blocks of four waves up to head_dim 64, two up to 128, one above; one block of eight
-        const int slots = hd > 128 || p.rows == 256 ? 256 : (hd <= 64 ? 768 : 512);
+        // what fits the CUs at once: four blocks of four waves up to head_dim 32 (16 heads, 8192 causal tokens: 195 us, 210 with three), three up to 64, two up to 128, one above; one block of
+        // eight
+        const int slots = hd > 128 || p.rows == 256 ? 256 : (hd <= 32 ? 1024 : hd <= 64 ? 768 : 512);
         const int64_t steps = (rows / p.rows + used) * Hkv * (((int64_t)max_keys + 63) / 64 + ITEM_COST);
         p.blocks = steps / MIN_SHARE >= slots ? slots : (int)((steps / MIN_SHARE + 8) / 8 * 8);
         p.cuts = p.blocks;
@@ -933,7 +940,7 @@ int launch(const PagedAttn& a, const Plan& p, hipStream_t st) {
     } else if (p.rows == 256) {
         if constexpr (HDP > 64 && HDP <= 128) launch_tile<HDP, 8, 4>(a, p.blocks, st);
     } else {
-        launch_tile<HDP, 4, (HDP <= 64 ? 3 : 2)>(a, p.blocks, st);
+        launch_tile<HDP, 4, 2>(a, p.blocks, st);
     }
     UFV_CHECK_LAUNCH();
     return UFV_OK;

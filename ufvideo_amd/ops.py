@@ -965,7 +965,11 @@ def rope_axes_table(inv_freq, positions, axis_of, out=None):
         _bad("inv_freq", "a dense fp32 vector", inv_freq)
     if positions.dtype is not _I64 or len(sh) != 2 or positions.get_device() != di or (positions.stride(1) != 1 and sh[1] > 1):
         _bad("positions", f"int64 [axes, N] on cuda:{di}", positions)
-    if len(axis_of) != half or min(axis_of) < 0 or max(axis_of) >= sh[0]:
+    try:
+        amap = bytes(tuple(axis_of))                                         # (the entry point compares every axis with their number)
+    except (TypeError, ValueError):
+        amap = b""
+    if len(amap) != half:
         raise _lib.UfvError(f"axis_of must name one of the {sh[0]} axes for each of the {half} pairs")
     N = sh[1]
     if out is None:
@@ -973,7 +977,7 @@ def rope_axes_table(inv_freq, positions, axis_of, out=None):
     else:
         _table(out, N, 2 * half, di, "out")
     if N:
-        _on_device(di, "ufv_rope_axes_table", inv_freq.data_ptr(), positions.data_ptr(), positions.stride(0), sh[0], bytes(axis_of), N, 2 * half, out.data_ptr())
+        _on_device(di, "ufv_rope_axes_table", inv_freq.data_ptr(), positions.data_ptr(), positions.stride(0), sh[0], amap, N, 2 * half, out.data_ptr())
     return out
 
 
