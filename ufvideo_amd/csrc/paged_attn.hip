@@ -632,67 +632,122 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : HDP > 32 ? 2 : 4) void att
 constexpr int TARGET = 448;
 constexpr int STEP_SH = 7;                 // log2 of the keys of a step: 4 waves x 32.  The shortest part is one step: one slot of 1000 tokens 10.2 us, 11.7 with two
 
-// What unit u of a head is: its tile, its keys [k0, k1) in steps, part of parts.  Every wave finds it for itself, a slot a lane, with one round of loads: sums the steps of the batch for the
-// length of a part, then the slots' units.
-__device__ __forceinline__ bool paged_unit(const PagedAttn& a, int u, PagedTile& w, int& part, int& parts, int& per, int& first) {
-    const int lane = threadIdx.x & 63;
+// What unit u of a head is: its tile, its keys [k0, k1) in steps, part of parts.  Every block finds it for itself: it sums the steps of the batch for the length of a part, then the slots'
+// units.  ALONE, up to 64 slots: every wave for itself, a slot a lane, no barrier (0.5 us less); else a slot a thread, 256 at a time (700 slots of 200 .. 1999 tokens 323 us, 353 with every wave
+// for itself; 200 of 50 .. 798 42 | 46).  (Longest parts first, by classes of length: no gain.)
+struct PUnitLds {
+    unsigned sum[4];
+    int scan[4][2];
+    int cu, n, len, s, parts, per, r, first;
+};
+template <int NW, bool ALONE>
+__device__ __forceinline__ bool paged_unit(const PagedAttn& a, PUnitLds& m, int u, PagedTile& w, int& part, int& parts, int& per, int& first) {
+    static_assert(NW == 4, "the LDS holds the sums of four waves");
+    constexpr int SPAN = ALONE ? 64 : NW * 64;                                         // slots of a round
+    const int tid = threadIdx.x, lane = tid & 63, wave = ALONE ? 0 : tid >> 6, me = ALONE ? lane : tid;
     int c0, n, len, tiles, steps;
     auto load = [&](int s0) {
-        const int s = min(s0 + lane, a.t.S - 1), c1 = a.t.cu_q[s + 1];
+        const int s = min(s0 + me, a.t.S - 1), c1 = a.t.cu_q[s + 1];
         c0 = a.t.cu_q[s];
         len = paged_len(a.t, s);
         n = c1 - c0;
-        const bool there = s0 + lane < a.t.S && c0 >= 0 && n > 0 && c1 <= a.N;
+        const bool there = s0 + me < a.t.S && c0 >= 0 && n > 0 && c1 <= a.N;
         tiles = there ? (n * a.G + 31) >> 5 : 0;
         steps = (int)(((unsigned)len + (1u << a.sh) - 1) >> a.sh);
     };
     unsigned all = 0;
-    for (int s0 = 0; s0 < a.t.S; s0 += 64) {
+    for (int s0 = 0; s0 < a.t.S; s0 += SPAN) {
         load(s0);
         all += (unsigned)tiles * (unsigned)steps;                                      // (below 2^31 over the batch: see `sh`)
     }
-    all = __builtin_amdgcn_readlane(lane_scan(all), 63);
-    const int length = a.target ? max((int)((all + a.target - 1) / a.target), 1) : 1 << 30;
-    int before = 0, cut = 0;                                                           // units, units of cut items of the slots before
-    for (int s0 = 0; s0 < a.t.S; s0 += 64) {
-        if (a.t.S > 64) load(s0);
-        const int most = max((steps + length - 1) / length, 1), p = max((steps + most - 1) / most, 1), k = max((steps + p - 1) / p, 1), mine = tiles * k, mc = k > 1 ? mine : 0;
-        const int x = lane_scan(mine), xc = lane_scan(mc), c = __popcll(__ballot(before + x <= u));
-        if (c == 64) {
-            before += __builtin_amdgcn_readlane(x, 63);
-            cut += __builtin_amdgcn_readlane(xc, 63);
-            continue;
-        }
-        parts = __builtin_amdgcn_readlane(k, c);
-        per = __builtin_amdgcn_readlane(p, c);
-        w.s = s0 + c;
-        w.q0 = __builtin_amdgcn_readlane(c0, c);
-        w.n = __builtin_amdgcn_readlane(n, c);
-        w.len = __builtin_amdgcn_readlane(len, c);
-        w.rows = w.n * a.G;
-        const int r = u - before - __builtin_amdgcn_readlane(x - mine, c);
-        if (r < 0) return false;                                                       // (cu_q that does not ascend: nothing outside the arrays is touched)
-        w.row0 = r / parts * 32;
-        part = r % parts;
-        first = cut + __builtin_amdgcn_readlane(xc - mc, c) + r - part;
-        return w.row0 < w.rows && (parts == 1 || (first >= 0 && (int64_t)(first + parts) * a.Hkv <= a.parts));
+    all = lane_scan(all);
+    if constexpr (ALONE) {
+        all = __builtin_amdgcn_readlane(all, 63);
+    } else {
+        if (lane == 63) m.sum[wave] = all;
+        if (tid == 0) m.parts = 0;
+        __syncthreads();
+        all = 0;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) all += m.sum[i];
     }
-    return false;
+    const int length = a.target ? max((int)((all + a.target - 1) / a.target), 1) : 1 << 30;
+    auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    int before = 0, cut = 0, r;                                                        // units, units of cut items of the slots before
+    for (int s0 = 0; s0 < a.t.S; s0 += SPAN) {
+        if (!ALONE && a.t.S > SPAN) load(s0);
+        const int most = max((steps + length - 1) / length, 1), p = max((steps + most - 1) / most, 1), k = max((steps + p - 1) / p, 1), mine = tiles * k, mc = k > 1 ? mine : 0;
+        const int x = lane_scan(mine), xc = lane_scan(mc);
+        if constexpr (ALONE) {
+            const int c = __popcll(__ballot(x <= u));                                  // the first lane whose units go past u
+            if (c == 64) return false;
+            auto of = [&](int v) { return __builtin_amdgcn_readlane(v, c); };
+            parts = of(k);
+            per = of(p);
+            w.s = c;
+            w.q0 = of(c0);
+            w.n = of(n);
+            w.len = of(len);
+            r = u - of(x - mine);
+            first = of(xc - mc);
+            if (r < 0) return false;
+        } else {
+            if (lane == 63) { m.scan[wave][0] = x; m.scan[wave][1] = xc; }
+            __syncthreads();
+            int b = before + x - mine, bc = cut + xc - mc;
+#pragma unroll
+            for (int i = 0; i < NW; ++i) {
+                b += i < wave ? m.scan[i][0] : 0;
+                bc += i < wave ? m.scan[i][1] : 0;
+                before += m.scan[i][0];
+                cut += m.scan[i][1];
+            }
+            if (u >= b && u < b + mine) {
+                m.cu = c0;
+                m.n = n;
+                m.len = len;
+                m.s = s0 + tid;
+                m.parts = k;
+                m.per = p;
+                m.r = u - b;
+                m.first = bc;
+            }
+            __syncthreads();
+            if (u < before) break;
+        }
+    }
+    if constexpr (!ALONE) {
+        parts = uni(m.parts);
+        if (parts == 0) return false;
+        per = uni(m.per);
+        w.s = uni(m.s);
+        w.q0 = uni(m.cu);
+        w.n = uni(m.n);
+        w.len = uni(m.len);
+        r = uni(m.r);
+        first = uni(m.first);
+    }
+    w.rows = w.n * a.G;
+    w.row0 = r / parts * 32;
+    part = r % parts;
+    first += r - part;
+    return w.row0 < w.rows && (parts == 1 || (first >= 0 && (int64_t)(first + parts) * a.Hkv <= a.parts));      // (cu_q that does not ascend: nothing outside the arrays is touched)
 }
 
-template <int HDP, int NW>
+template <int HDP, int NW, bool ALONE>
 __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_keys_k(PagedAttn a) {
     using C = PCfg<HDP>;
     constexpr int HALF = 32 * C::P, STAGE = 2 * HALF;
     static_assert(STAGE >= 32 * HDP * 4, "a wave's O fits its staging area");
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ float wm[NW][32], wl[NW][32];
+    __shared__ PUnitLds unit;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = lane >> 5, l31 = lane & 31, id = blockIdx.x;
     PagedTile w = {};
     int part = 0, parts = 0, per = 0, first = 0;
     w.g = id % a.Hkv;
-    const bool work = paged_unit(a, id / a.Hkv, w, part, parts, per, first);
+    const bool work = paged_unit<NW, ALONE>(a, unit, id / a.Hkv, w, part, parts, per, first);
     if (!work) return;
     if (a.target && tid == 0 && part == 0) {                                           // the item's record is at its number
         PCut* c = paged_cut(a) + (int64_t)(paged_number<32>(a.G, w.s, w.q0) + (w.row0 >> 5)) * a.Hkv + w.g;
@@ -793,15 +848,15 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_keys_k(
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
-// Does tile number t of 32 rows exist, that is, was its record written?  (a slot a lane)
+// Does tile number t of 32 rows exist, that is, was its record written?  (a slot a lane, above 64 slots a slot a thread; the answer of one counts)
 __device__ __forceinline__ bool paged_tile_exists(const PagedAttn& a, int t) {
-    const int lane = threadIdx.x & 63;
+    const bool alone = a.t.S <= 64;
     bool is = false;
-    for (int s0 = 0; s0 < a.t.S; s0 += 64) {
-        const int s = min(s0 + lane, a.t.S - 1), c0 = a.t.cu_q[s], c1 = a.t.cu_q[s + 1], row0 = (t - paged_number<32>(a.G, s, c0)) * 32;
-        is |= s0 + lane < a.t.S && c0 >= 0 && c1 > c0 && c1 <= a.N && row0 >= 0 && row0 < (c1 - c0) * a.G;
+    for (int s = alone ? threadIdx.x & 63 : threadIdx.x; s < a.t.S; s += 256) {
+        const int c0 = a.t.cu_q[s], c1 = a.t.cu_q[s + 1], row0 = (t - paged_number<32>(a.G, s, c0)) * 32;
+        is |= c0 >= 0 && c1 > c0 && c1 <= a.N && row0 >= 0 && row0 < (c1 - c0) * a.G;
     }
-    return __any(is);
+    return alone ? __any(is) : __syncthreads_or(is);
 }
 
 // The join of cut items.  blockIdx.x: the item's record.  A thread adds one quad of dims of one row over the parts, in their order, with weights 2^(m_p - m); eight lanes
@@ -930,12 +985,18 @@ void launch_tile(const PagedAttn& a, int blocks, hipStream_t st) {
     hipLaunchKernelGGL((attn_paged_join_k<HDP, 32 * NW, 1>), dim3(blocks, 32 * NW * (HDP / 4) / 256), dim3(256), 0, st, a);
 }
 
+template <int HDP, bool ALONE>
+void launch_keys(const PagedAttn& a, int blocks, hipStream_t st) {
+    constexpr int NW = 4, smem = NW * 64 * PCfg<HDP>::P;
+    UFV_ONCE_PER_DEVICE((void)hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_keys_k<HDP, NW, ALONE>), hipFuncAttributeMaxDynamicSharedMemorySize, smem););
+    hipLaunchKernelGGL((attn_paged_keys_k<HDP, NW, ALONE>), dim3(blocks), dim3(NW * 64), smem, st, a);
+}
+
 template <int HDP>
 int launch(const PagedAttn& a, const Plan& p, hipStream_t st) {
     if (p.keys) {
-        constexpr int NW = 4, smem = NW * 64 * PCfg<HDP>::P;
-        UFV_ONCE_PER_DEVICE((void)hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_keys_k<HDP, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, smem););
-        hipLaunchKernelGGL((attn_paged_keys_k<HDP, NW>), dim3(p.blocks), dim3(NW * 64), smem, st, a);
+        if (a.t.S <= 64) launch_keys<HDP, true>(a, p.blocks, st);
+        else launch_keys<HDP, false>(a, p.blocks, st);
         if (p.target) hipLaunchKernelGGL((attn_paged_join_k<HDP, 32, 4>), dim3(a.tiles * a.Hkv, HDP / 32), dim3(256), 0, st, a);
     } else if (p.rows == 256) {
         if constexpr (HDP > 64 && HDP <= 128) launch_tile<HDP, 8, 4>(a, p.blocks, st);
@@ -963,7 +1024,7 @@ extern "C" int ufv_attention_paged(const void* q, int64_t ldq, void* o, int64_t 
     UFV_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)o % 16 == 0 && ldq % 8 == 0 && ldo % 8 == 0, "ufv_attention_paged: rows must be 16-byte aligned (pitches %lld, %lld)", (long long)ldq,
                 (long long)ldo);
     UFV_REQUIRE(ldkv >= 2 * (int64_t)Hkv * hd && ldkv < 1 << 24 && (N == 1 || (ldq >= (int64_t)Hq * hd && ldo >= (int64_t)Hq * hd)), "ufv_attention_paged: a row pitch is out of range");
-    UFV_REQUIRE((int64_t)N * Hq < 0x7fffffff && S < 1 << 24, "ufv_attention_paged: too many rows or slots (N=%d S=%d)", N, S);
+    UFV_REQUIRE((int64_t)N * Hq < 0x7fffffff && S <= 65536, "ufv_attention_paged: too many rows or slots (N=%d S=%d)", N, S);
     const Plan p = make_plan(N, S, Hq, Hkv, hd, max_pages << paged_log2(page));
     UFV_REQUIRE(((int64_t)p.tiles + 2 * p.target) * Hkv < 0x7fffffff && Hkv < 65536, "ufv_attention_paged: too many row tiles (N=%d S=%d)", N, S);
     UFV_REQUIRE(p.ws == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= p.ws), "ufv_attention_paged: a 16-byte aligned workspace of %lld bytes is needed (%lld given)", (long long)p.ws,
