@@ -595,3 +595,71 @@ def test_attention_paged_new_workspace_contents_do_not_show():
             torch.cuda.synchronize()
             outs.append(out)
         assert all(torch.equal(outs[0], o) for o in outs) and outs[0].abs().max() > 0
+
+
+@pytest.mark.parametrize("Hq,Hkv,hd", [(28, 4, 128), (4, 2, 64)])
+def test_attention_paged_captured_with_changing_lengths(Hq, Hkv, hd):
+    """one graph per number of rows, replayed while cu_q, kv_len and the table change on the device: every replay equals the eager call, rows behind cu_q[S] stay"""
+    page, S, cap = 64, 3, 5000
+    for N, steps in ((400, ([300, 5, 95], [10, 200, 190], [1, 1, 1], [0, 400, 0], [0, 0, 0], [133, 133, 134])), (3, ([1, 1, 1], [0, 3, 0], [0, 0, 0], [2, 0, 1]))):
+        b = Batch([N, 0, 0], [cap] * 3, Hkv, hd, page, seed=N, device=DEV)
+        table, cu_q, kv_len = b.table.clone(), b.cu_q.clone(), b.kv_len.clone()
+        q, out = rnd(N, Hq * hd).to(BF), torch.zeros(N, Hq * hd, device=DEV, dtype=BF)
+        run = lambda o: ops.attention_paged(q, b.pages, table, cu_q, kv_len, Hq, Hkv, hd, out=o)
+        run(out)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            run(out)
+        for i, n in enumerate(steps * 2):
+            cu_q.copy_(i32([0, n[0], n[0] + n[1], sum(n)]))
+            kv_len.copy_(i32([(977 * (i + s) + n[s]) % (cap - N) + n[s] for s in range(S)]))
+            table.copy_(b.table.roll(i, 0))
+            out.fill_(7.0)
+            eager = torch.full_like(out, 7.0)
+            g.replay()
+            run(eager)
+            if i % 3 == 0:
+                torch.cuda.synchronize()
+            assert torch.equal(out, eager) and (out[sum(n):] == 7.0).all() and not (sum(n) and (out[:sum(n)] == 7.0).all()), (N, i)
+
+
+def test_compaction_captured_into_a_graph():
+    S, page, L, P, width = 5, 16, 2, 60, 64
+    states = []
+    for _ in range(2):
+        states.append(dict(pool=rnd(L, P, page, width, seed=3).to(BF), table=torch.full((S, 12), -1, dtype=torch.int32, device=DEV), lens=i32([0] * S), refs=i32([0] * P),
+                           grow=i32([33, 17, 60, 5, 40]), drop=i32([0, 1, 0, 0, 1])))
+
+    def turn(st):
+        granted, cu_q, pairs = ops.kv_pages_extend(st["table"], st["lens"], st["refs"], st["grow"], page)
+        ops.kv_pages_copy(st["pool"], pairs)
+        ops.kv_pages_free(st["table"], st["lens"], st["refs"], st["drop"], page)
+        st["counts"] = ops.kv_pages_compact(st["pool"], st["table"], st["lens"], st["refs"])
+
+    for st in states:
+        turn(st)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        turn(states[0])
+    captured = states[0]["counts"]
+    for i in range(8):
+        for st in states:
+            st["drop"].copy_(i32([(i + s) % 3 == 0 for s in range(S)]))
+        g.replay()
+        turn(states[1])
+        if i % 3 == 0:
+            torch.cuda.synchronize()
+        for k in ("table", "lens", "refs", "pool"):
+            assert torch.equal(states[0][k], states[1][k]), (i, k)
+        assert torch.equal(captured, states[1]["counts"])
+        live = int(captured[0])
+        assert (states[0]["refs"][:live] > 0).all() and not states[0]["refs"][live:].any()
+
+
+def test_rope_axes_table_refuses_axes_that_do_not_exist():
+    inv, pos = torch.ones(32, device=DEV), torch.zeros(3, 4, dtype=torch.int64, device=DEV)
+    for bad in (32, [0] * 31, [0] * 33, [-1] + [0] * 31, [3] + [0] * 31, [300] + [0] * 31, ["x"] * 32, None):
+        with pytest.raises(_lib.UfvError):
+            ops.rope_axes_table(inv, pos, bad)
