@@ -1033,7 +1033,7 @@ def attention_paged(q, pages, block_table, cu_q, kv_len, Hq, Hkv, hd, scale=None
     dst, ldo = _rows(out, N, Hq * hd, di, "out")
     if N:
         nbytes = _attention_paged_ws(N, pa[9], Hq, Hkv, hd, min(pa[6] * pa[2], 0x7fffffff))
-        ws = torch.empty((nbytes,), device=q.device, dtype=torch.uint8) if nbytes > 0 else None       # the caching allocator's: private to this call, also inside a captured graph
+        ws = kv_len.new_empty((nbytes + 3) >> 2) if nbytes > 0 else None       # the caching allocator's: private to this call, also inside a captured graph
         _on_device(di, "ufv_attention_paged", src, ldq, dst, ldo, N, Hq, Hkv, hd, *pa, hd ** -0.5 if scale is None else scale, int(causal), 0 if ws is None else ws.data_ptr(), nbytes)
     return out
 
@@ -1057,7 +1057,7 @@ def kv_pages_extend(block_table, kv_len, refs, n_new, page):
     `kv_pages_copy(pool, pairs)` must follow before the new tokens are appended: pairs name the shared last pages that slots got a page of their own for."""
     di, S, P, a = _table_args(block_table, kv_len, refs, page)
     nn = _vec(n_new, S, di, "n_new")
-    granted, cu_q, pairs, ws = torch.empty((8 * S + 1 + P,), device=block_table.device, dtype=_I32).split((S, S + 1, 3 * S, 3 * S + P))
+    granted, cu_q, pairs, ws = block_table.new_empty(8 * S + 1 + P).split_with_sizes((S, S + 1, 3 * S, 3 * S + P))
     _on_device(di, "ufv_kv_pages_extend", *a, nn, granted.data_ptr(), cu_q.data_ptr(), pairs.data_ptr(), ws.data_ptr(), 4 * (3 * S + P))
     return granted, cu_q, pairs.view(S, 3)
 
@@ -1092,6 +1092,6 @@ def kv_pages_compact(pool, block_table, kv_len, refs):
     di, S, P, a = _table_args(block_table, kv_len, refs, page)
     if dp != di or NP != P:
         raise _lib.UfvError(f"refs must have one entry for each of the pool's {NP} pages ({P}), tables and pool live on one device")
-    counts, ws = torch.empty((2 + 3 * P,), device=pool.device, dtype=_I32).split((2, 3 * P))
+    counts, ws = block_table.new_empty(2 + 3 * P).split_with_sizes((2, 3 * P))
     _on_device(di, "ufv_kv_pages_compact", ptr, L, lb, rb, *a, counts.data_ptr(), ws.data_ptr(), 12 * P)
     return counts
