@@ -202,7 +202,6 @@ def load():
 
 
 def call(name, *args):
-    lib = load()
-    rc = getattr(lib, name)(*args)
+    rc = getattr(_lib or load(), name)(*args)
     if rc != 0:
-        raise UfvError(f"{name} failed ({rc}): {lib.ufv_last_error().decode()}")
+        raise UfvError(f"{name} failed ({rc}): {_lib.ufv_last_error().decode()}")

@@ -905,11 +905,14 @@ def mask_loss_bwd(x, t, coef, cb):
 _BF, _F32, _I32, _I64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
 
 
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _on_device(di, name, *args):
-    if di == torch.cuda.current_device():
-        return _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(di))
+    if di == _current_device():
+        return _lib.call(name, *args, _raw_stream(di))
     with torch.cuda.device(di):
-        return _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(di))
+        return _lib.call(name, *args, _raw_stream(di))
 
 
 def _bad(name, want, t):
@@ -925,7 +928,7 @@ def _gpu_index(t, name):
 
 def _vec(t, n, di, name):
     """int32 vector of n entries -> its address"""
-    if t.dtype is not _I32 or t.get_device() != di or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+    if t.dtype is not _I32 or t.get_device() != di or t.shape != (n,) or not t.is_contiguous():
         _bad(name, f"a dense int32 vector of {n} entries on cuda:{di}", t)
     return t.data_ptr()
 
