@@ -148,12 +148,14 @@ __device__ __forceinline__ void paged_step(const char* __restrict__ kb, const ch
     for (int hh = 0; hh < NH; ++hh)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[hh][r] = 0.f;
+    // NH = 2: a wave among its products goes before one among its exponentials (two of different blocks on a SIMD: 8 x 1000 causal tokens 126 -> 121 us, 16 questions 59 -> 56)
     {
         bf16x8 kf[PRE];
         auto read = [&](int i) { return *reinterpret_cast<const bf16x8*>(kb + (k_off ^ ((i / NH) << 5)) + (i % NH) * 32 * C::P); };
 #pragma unroll
         for (int i = 0; i < PRE; ++i) kf[i] = read(i);
         __builtin_amdgcn_sched_barrier(0);
+        if (NH == 2) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
             s[i % NH] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i % PRE], qf[i / NH], s[i % NH], 0, 0, 0);
@@ -162,6 +164,7 @@ __device__ __forceinline__ void paged_step(const char* __restrict__ kb, const ch
             __builtin_amdgcn_sched_barrier(0);
         }
     }
+    if (NH == 2) __builtin_amdgcn_s_setprio(0);
     if (hide) {
         const int lim = vis - 4 * h;
 #pragma unroll
@@ -207,6 +210,7 @@ __device__ __forceinline__ void paged_step(const char* __restrict__ kb, const ch
     };
     exps(0, 0, 16);
     bf16x8 pf[2];
+    if (NH == 2) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         if (i % NM == 0) {
@@ -225,6 +229,7 @@ __device__ __forceinline__ void paged_step(const char* __restrict__ kb, const ch
         if (NH == 2 && i < NM) exps(1, EPM * i < 16 ? EPM * i : 16, EPM * (i + 1) < 16 ? EPM * (i + 1) : 16);
         __builtin_amdgcn_sched_barrier(0);
     }
+    if (NH == 2) __builtin_amdgcn_s_setprio(0);
     st.l += sum;
 }
 
