@@ -663,3 +663,55 @@ def test_rope_axes_table_refuses_axes_that_do_not_exist():
     for bad in (32, [0] * 31, [0] * 33, [-1] + [0] * 31, [3] + [0] * 31, [300] + [0] * 31, ["x"] * 32, None):
         with pytest.raises(_lib.UfvError):
             ops.rope_axes_table(inv, pos, bad)
+
+
+def test_operators_on_parts_of_larger_tables_and_pools():
+    """rows and columns of a larger table, slots of longer vectors, layers and columns of larger tensors: what lies beside them stays"""
+    S, W, page, Hkv, Hq, hd, L = 3, 9, 16, 2, 4, 64, 2
+    P, width = 40, 2 * Hkv * hd
+    big_table = torch.full((S + 3, W + 4), 99, dtype=torch.int32, device=DEV)
+    big_len, big_refs = i32([77] * (S + 2)), i32([0] * P)
+    big_pool = rnd(L + 2, P, page, width, seed=1).to(BF)
+    table, lens, pool = big_table[1:S + 1, 2:W + 2], big_len[1:S + 1], big_pool[1:L + 1]
+    table.fill_(-1)
+    lens.zero_()
+    alone = dict(table=table.clone(), lens=lens.clone(), refs=big_refs.clone(), pool=pool.clone())
+    qkv = rnd(60, (Hq + 2 * Hkv) * hd + 8, seed=2).to(BF)
+    tab = rnd(60, hd, seed=3)
+    outs = []
+    for st in (dict(table=table, lens=lens, refs=big_refs, pool=pool), alone):
+        x = qkv.clone()
+        got = []
+        for turn, (grow, parent, drop) in enumerate((([20, 0, 31], [-1, 0, -1], [0, 0, 0]), ([5, 7, 1], [-1, -1, -1], [0, 0, 1]), ([30, 2, 9], [-1, -1, -1], [1, 0, 0]))):
+            granted, cu_q, pairs = ops.kv_pages_extend(st["table"], st["lens"], st["refs"], i32(grow), page)
+            ops.kv_pages_copy(st["pool"], pairs)
+            n = sum(grow)
+            rows = x[:n].clone()
+            for l in range(L):
+                q = ops.rope_kv_paged(rows.clone(), tab[:n], Hq, Hkv, hd, st["pool"][l], st["table"], cu_q, st["lens"])
+                got.append(ops.attention_paged(q, st["pool"][l], st["table"], cu_q, st["lens"], Hq, Hkv, hd))
+            ops.kv_pages_fork(st["table"], st["lens"], st["refs"], i32(parent), page)
+            ops.kv_pages_free(st["table"], st["lens"], st["refs"], i32(drop), page)
+            got.append(ops.kv_pages_compact(st["pool"], st["table"], st["lens"], st["refs"]))
+        outs.append(got)
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    assert torch.equal(table, alone["table"]) and torch.equal(lens, alone["lens"]) and torch.equal(big_refs, alone["refs"]) and torch.equal(pool, alone["pool"])
+    inside = torch.zeros_like(big_table, dtype=torch.bool)
+    inside[1:S + 1, 2:W + 2] = True
+    assert (big_table[~inside] == 99).all() and big_len[0] == 77 and big_len[S + 1] == 77
+    fresh = rnd(L + 2, P, page, width, seed=1).to(BF)
+    assert torch.equal(big_pool[0], fresh[0]) and torch.equal(big_pool[-1], fresh[-1])
+
+
+def test_operators_without_rows():
+    S, page, Hkv, Hq, hd = 2, 16, 1, 2, 32
+    pages = rnd(4, page, 2 * Hkv * hd).to(BF)
+    table, cu_q, kv_len = i32([[0, 1], [2, 3]]), i32([0, 0, 0]), i32([5, 0])
+    keep = pages.clone()
+    q = ops.rope_kv_paged(torch.empty(0, (Hq + 2 * Hkv) * hd, device=DEV, dtype=BF), torch.empty(0, hd, device=DEV), Hq, Hkv, hd, pages, table, cu_q, kv_len)
+    assert q.shape == (0, Hq * hd) and ops.attention_paged(q, pages, table, cu_q, kv_len, Hq, Hkv, hd).shape == (0, Hq * hd)
+    assert ops.rope_axes_table(torch.ones(16, device=DEV), torch.zeros(2, 0, dtype=torch.int64, device=DEV), [0] * 16).shape == (0, 32)
+    x = torch.full((7, Hq * hd), 2.0, device=DEV, dtype=BF)                    # rows, but of no slot
+    out = torch.full_like(x, 3.0)
+    ops.attention_paged(x, pages, table, cu_q, kv_len, Hq, Hkv, hd, out=out)
+    assert (out == 3.0).all() and torch.equal(pages, keep)
