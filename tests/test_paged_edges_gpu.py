@@ -1,0 +1,72 @@
+"""GPU: what the paged-cache operators make of infinities and NaN that a row does see, and of views whose strides say nothing (an axis of one entry, one set of positions for all axes).
+Finite results are compared with the 64-bit oracle's bound element by element, the others have to be the same kind of value."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from paged_ref import Batch, attend  # noqa: E402
+from ufvideo_amd import ops  # noqa: E402
+
+DEV = "cuda"
+BF = torch.bfloat16
+INF, NAN = float("inf"), float("nan")
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def rnd(*shape, seed=0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(DEV)
+
+
+def same_kind(got, want, slack, what=""):
+    """+inf, -inf and NaN in the same places, the rest within slack"""
+    got = got.double()
+    for name, f in (("nan", torch.isnan), ("+inf", torch.isposinf), ("-inf", torch.isneginf)):
+        d = f(got) != f(want)
+        assert not d.any(), f"{what}: {name} differs in {int(d.sum())} places, first {d.nonzero()[0].tolist()}: {got[d][0]} for {want[d][0]}"
+    ok = torch.isfinite(want)
+    bad = ok & ~((got - want).abs() <= slack)
+    assert not bad.any(), f"{what}: {int(bad.sum())} elements off, at {bad.nonzero()[0].tolist()}"
+
+
+# ---- V alone ----------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("Hq,Hkv,hd", [(4, 2, 128), (4, 2, 64), (2, 1, 32), (3, 1, 72), (2, 1, 192)])
+@pytest.mark.parametrize("q,kv", [(1, 50), (3, 50), (20, 90), (5, 700), (40, 40), (150, 1517), (300, 300), (20, 13)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_paged_bad_elements_of_v_reach_the_rows_that_see_them(Hq, Hkv, hd, q, kv, causal):
+    """one V row at a time holds +inf, -inf and NaN, K is finite: before the new tokens (in the step of the first of them and in earlier ones), at the first, among them, at the last"""
+    b = Batch([q, 1], [kv, 40], Hkv, hd, 16, seed=hd, device=DEV)
+    x = rnd(b.N, Hq * hd, seed=q).to(BF)
+    clean, first, v0 = b.pages.clone(), max(kv - q, 0), (2 * Hkv - 1) * hd        # V of the last kv head
+    for at in sorted({0, first // 64 * 64, first // 32 * 32, max(first - 1, 0), first, min(first + 1, kv - 1), (first + kv) // 2, kv - 1}):
+        b.pages.copy_(clean)
+        for d, bad in ((0, INF), (5, -INF), (hd - 1, NAN)):
+            b.pages[b.row(0, at)][v0 + d] = bad
+        if at > 0:                                                                # both signs in one column: NaN where a row sees both
+            b.pages[b.row(0, at - 1)][v0 + 3], b.pages[b.row(0, at)][v0 + 3] = INF, -INF
+        got = ops.attention_paged(x, b.pages, b.table, b.cu_q, b.kv_len, Hq, Hkv, hd, causal=causal)
+        want, slack = attend(b, x, Hq, causal=causal)
+        assert not torch.isfinite(want).all()
+        same_kind(got, want, slack, f"V row {at} of {kv}, {q} new")
+
+
+@pytest.mark.parametrize("q,kv,Hq,Hkv,hd", [(24, 9000, 28, 4, 128), (300, 4000, 7, 1, 128), (700, 2050, 3, 1, 128), (2100, 2100, 1, 1, 72)])
+def test_attention_paged_bad_elements_of_v_in_cut_items(q, kv, Hq, Hkv, hd):
+    """the same where several blocks work on the item, and in the middle of a whole prompt of several tiles"""
+    b = Batch([q], [kv], Hkv, hd, 64, seed=1, device=DEV)
+    x = rnd(q, Hq * hd, seed=2).to(BF)
+    want0, slack0 = attend(b, x, Hq)
+    first, v0 = kv - q, (2 * Hkv - 1) * hd
+    for at in sorted({10, first // 64 * 64, max(first - 1, 0), first, first + 1, (first + kv) // 2, kv - 1}):
+        kept = b.pages[b.row(0, at)].clone()
+        for d, bad in ((1, INF), (6, -INF), (hd - 1, NAN)):
+            b.pages[b.row(0, at)][v0 + d] = bad
+        got = ops.attention_paged(x, b.pages, b.table, b.cu_q, b.kv_len, Hq, Hkv, hd)
+        b.pages[b.row(0, at)] = kept
+        want = want0.view(q, Hkv, Hq // Hkv, hd).clone()                          # every weight of a seen key is above 0: its column is the bad value
+        for d, bad in ((1, INF), (6, -INF), (hd - 1, NAN)):
+            want[max(at - first, 0):, -1, :, d] = bad
+        same_kind(got, want.view(q, -1), slack0, f"V row {at} of {kv}, {q} new")

@@ -235,7 +235,7 @@ __device__ __forceinline__ void paged_step(const char* __restrict__ kb, const ch
 
 // A key that a row does not see must not reach it even when its V row holds Inf or NaN (0 * Inf in the matrix product): among the new tokens of a causal chunk -- the only keys
 // that some rows see and others do not -- such elements are staged as zeros, and if there was one, they are added after the walk to the rows that see them (keys j0 .. j1 - 1;
-// p > 0 times Inf or NaN is Inf or NaN).
+// p > 0 times Inf or NaN is Inf or NaN).  Whole steps are cleaned, so the range begins at the first key of the step that holds the first new token, not at that token.
 template <int HDP>
 __device__ __forceinline__ void paged_add_bad(const PagedAttn& a, const PagedTile& w, int j0, int j1, PState<HDP>& st, int seen) {
     int h = (threadIdx.x & 63) >> 5;
@@ -619,7 +619,7 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : HDP > 32 ? 2 : 4) void att
             if (bad) dirty = 1;
             __syncthreads();
             if (dirty) {
-                paged_add_bad<HDP>(a, w, max(diag, t0 << 6), min(t1 << 6, w.len), st, seen);
+                paged_add_bad<HDP>(a, w, max(max(diag, 0) & ~63, t0 << 6), min(t1 << 6, w.len), st, seen);
                 __syncthreads();
                 if (tid == 0) dirty = 0;                                                // (the next item sets it behind barriers of its own)
             }
@@ -815,7 +815,7 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_keys_k(
         __builtin_amdgcn_wave_barrier();
     }
     if (dirty)
-        for (int t = t0 + wave; t < t1; t += NW) paged_add_bad<HDP>(a, w, max(diag, t << 5), min((t + 1) << 5, w.len), st, seen);
+        for (int t = t0 + wave; t < t1; t += NW) paged_add_bad<HDP>(a, w, max(max(diag, 0) & ~31, t << 5), min((t + 1) << 5, w.len), st, seen);
     // ---- join the waves: (m, l) and O [row][HDP] of every wave through LDS, then every thread sums quads of the rows that exist
     const float l = st.l + __shfl_xor(st.l, 32, 64);
     if (h == 0) { wm[wave][l31] = st.m; wl[wave][l31] = l; }
