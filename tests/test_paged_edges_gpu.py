@@ -70,3 +70,25 @@ def test_attention_paged_bad_elements_of_v_in_cut_items(q, kv, Hq, Hkv, hd):
         for d, bad in ((1, INF), (6, -INF), (hd - 1, NAN)):
             want[max(at - first, 0):, -1, :, d] = bad
         same_kind(got, want.view(q, -1), slack0, f"V row {at} of {kv}, {q} new")
+
+
+# ---- scores of -inf ---------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("hd", [8, 16, 40, 64, 72, 80, 104, 128, 192, 256])
+@pytest.mark.parametrize("q,kv", [(1, 70), (3, 200), (150, 300), (2100, 2100)])
+def test_attention_paged_a_key_of_weight_nothing_leaves_its_row_finite(hd, q, kv):
+    """K elements of -inf: rows whose q has the sign that makes the score -inf go on without the key, the others become NaN -- at every head_dim, full register width or not"""
+    Hq, Hkv, page = 2, 1, 64
+    junk = torch.full((4, page, 2 * Hkv * hd), NAN, device=DEV, dtype=BF)            # what ran before leaves NaN in the chip's memories
+    junk_rows = max(q * Hq // 2, 1)
+    ops.attention_paged(torch.ones(junk_rows, Hq * hd, device=DEV, dtype=BF), junk, i32([[0, 1, 2, 3]]), i32([0, junk_rows]), i32([200]), Hq, Hkv, hd)
+    b = Batch([q], [kv], Hkv, hd, page, seed=hd, device=DEV)
+    x = rnd(q, Hq * hd, seed=3).to(BF)
+    for j, d in ((1, 0), (kv // 2, 7), (kv - 1, hd - 1)):
+        b.pages[b.row(0, j)][d] = -INF
+    xh = x.view(q, Hq, hd)[:(q + 1) // 2]
+    xh[:, :, [0, 7, hd - 1]] = xh[:, :, [0, 7, hd - 1]].abs() + 0.125
+    got = ops.attention_paged(x, b.pages, b.table, b.cu_q, b.kv_len, Hq, Hkv, hd)
+    want, slack = attend(b, x, Hq)
+    alone = torch.isnan(want.view(q, Hq, hd)).all(-1, keepdim=True).expand(q, Hq, hd).reshape(q, -1)
+    assert (q <= 2 or not alone.all()) and torch.equal(alone, torch.isnan(want))
+    same_kind(got, want, slack, f"hd {hd}, {q} new of {kv}")

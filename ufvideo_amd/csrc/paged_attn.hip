@@ -288,10 +288,16 @@ __device__ __forceinline__ int paged_load_q(const PagedAttn& a, const PagedTile&
     return paged_seen(a, w.len, w.n, tok);
 }
 
+// A lane's place in a load of rows (see PFetch): chunk sch of row srow.  Lanes whose chunk lies behind hd (padded head dims) ask for a place behind every range and get zeros: Q is 0 there, but
+// so must K be (0 * Inf is NaN: a finite row with one score of -inf would become NaN).  A range has fewer than 2^29 bytes: 16 rows, ldkv below 2^24.
+__device__ __forceinline__ unsigned paged_lane_offset(const PagedAttn& a, int srow, int sch) {
+    return sch * 8 < a.hd ? (unsigned)(srow * (int)a.ldkv + sch * 8) * 2 : 0x7ffffff0u;
+}
+
 // Fetching NG groups of 16 keys (a step) by NWS waves.  A wave load covers RPW <= 16 rows that start at a multiple of RPW, and a page holds whole groups of 16 tokens: the page is the same
 // for the whole load and its address a scalar; the lane's part of the address does not change.  It is a buffer load whose base is the load's first row and whose range ends behind the last row
-// that is a key: what lies outside -- tokens behind the last one, a page outside the pool -- comes back as zeros and is not read.  Lanes whose chunk lies behind hd (padded head dims) fetch
-// chunk 0: their K meets zeros in Q, their V columns are not stored.  Page ids: one vector load holds those of 64 groups, one a lane.
+// that is a key: what lies outside -- tokens behind the last one, a page outside the pool -- comes back as zeros and is not read.  Page ids: one vector load
+// holds those of 64 groups, one a lane.
 template <int HDP, int NG, int NWS>
 struct PFetch {
     using C = PCfg<HDP>;
@@ -510,7 +516,7 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : HDP > 32 ? 2 : 4) void att
     PWalk<R, NW * 64> walk;
     if (!walk.start(a, shared)) return;
     const int srow = lane / C::CPR, sch = (lane % C::CPR) ^ C::f(wave * C::RPW + srow);  // the lane's row in a load, the chunk that belongs into its place
-    const unsigned lane_off = (unsigned)(srow * (int)a.ldkv + (sch * 8 < a.hd ? sch * 8 : 0)) * 2;
+    const unsigned lane_off = paged_lane_offset(a, srow, sch);
 
     using F = PFetch<HDP, 4, NW>;
     constexpr int NL = F::NL, D = NS - 1;                                              // steps ahead
@@ -768,7 +774,7 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_keys_k(
     char* kb = smem + wave * STAGE;
     char* vb = kb + HALF;
     const int srow = lane / C::CPR, sch = lane % C::CPR;
-    const unsigned lane_off = (unsigned)(srow * (int)a.ldkv + (sch * 8 < a.hd ? sch * 8 : 0)) * 2;
+    const unsigned lane_off = paged_lane_offset(a, srow, sch);
     const int diag = a.causal && w.n > 1 ? w.len - w.n : 0x7fffffff;
     using F = PFetch<HDP, 2, 1>;
     F fe;
