@@ -548,7 +548,8 @@ UFV_API int ufv_rope_rows_table(const void* x, int64_t ldx, void* y, int64_t ldy
 /* RoPE + append: row n of qkv bf16 [N, ldqkv] = [q | k | v] heads -> q_out[n] = rotated q (may be the q columns of qkv), the row's cache row = [rotated k | v].  hd % 16 == 0 */
 UFV_API int ufv_rope_kv_paged(const void* qkv, int64_t ldqkv, void* q_out, int64_t ldq, int N, int Hq, int Hkv, int hd, const float* table, void* pages, int n_pages, int page,
                               int64_t ldkv, const int32_t* block_table, int64_t ld_table, int max_pages, const int32_t* cu_q, const int32_t* kv_len, int S, void* stream);
-/* o[n] = softmax(q k^T * scale) v of every packed row over its slot's cached tokens (causal: up to the row's own), GQA, fp32 softmax; a row that sees no key gets zeros.
+/* o[n] = softmax(q k^T * scale) v of every packed row over its slot's cached tokens (causal: up to the row's own), GQA, fp32 softmax; a row that sees no key gets zeros,
+ * a row all of whose keys score -inf NaN.
  * q, o bf16, head h at column h*hd; hd a multiple of 8 up to 256; scale positive and finite; ldkv below 2^24.  cu_q must ascend.  ws, 16-byte aligned, of any content: ufv_attention_paged_ws_bytes(N, S, Hq, Hkv, hd, max_pages * page) bytes (may be 0), not shared by
  * calls that can run at the same time. */
 UFV_API int64_t ufv_attention_paged_ws_bytes(int N, int S, int Hq, int Hkv, int hd, int max_keys);

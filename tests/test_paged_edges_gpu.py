@@ -92,3 +92,53 @@ def test_attention_paged_a_key_of_weight_nothing_leaves_its_row_finite(hd, q, kv
     alone = torch.isnan(want.view(q, Hq, hd)).all(-1, keepdim=True).expand(q, Hq, hd).reshape(q, -1)
     assert (q <= 2 or not alone.all()) and torch.equal(alone, torch.isnan(want))
     same_kind(got, want, slack, f"hd {hd}, {q} new of {kv}")
+
+
+def defined(b, q, Hq, causal):
+    """the definition, a row at a time in 64 bits: softmax over the scores of the keys that the row sees; zeros where there is none"""
+    hd, G = b.hd, Hq // b.Hkv
+    o = torch.zeros(q.shape[0], Hq, hd, dtype=torch.float64)
+    pages, x = b.pages.cpu().double(), q.cpu().double().view(q.shape[0], Hq, hd)
+    for s, (n, kv) in enumerate(zip(b.q_lens, b.kv_lens)):
+        for r in range(n):
+            keys = [b.row(s, j) for j in range(min(kv, kv - n + r + 1) if causal else kv)]
+            keys = [k for k in keys if k is not None]
+            if not keys:
+                continue
+            rows = pages[torch.tensor([k[0] for k in keys]), torch.tensor([k[1] for k in keys])]
+            for h in range(Hq):
+                g = h // G
+                p = torch.softmax((rows[:, g * hd:(g + 1) * hd] * x[b.cu[s] + r, h]).sum(1) * hd ** -0.5, 0)
+                o[b.cu[s] + r, h] = (p[:, None] * rows[:, (b.Hkv + g) * hd:(b.Hkv + g + 1) * hd]).sum(0)
+    return o.view(q.shape[0], -1).to(q.device)
+
+
+@pytest.mark.parametrize("q_lens,kv_lens,Hq,Hkv,hd", [([1, 1], [70, 20], 4, 2, 64), ([1, 1], [9000, 700], 4, 2, 128), ([5, 3], [9, 2], 4, 2, 72), ([40, 1], [60, 33], 4, 2, 128),
+                                                      ([40], [13], 4, 2, 64), ([70, 9], [2100, 9], 2, 1, 128), ([1] * 70, [30] * 70, 2, 2, 32)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_paged_rows_of_nothing_but_scores_of_minus_infinity(q_lens, kv_lens, Hq, Hkv, hd, causal):
+    """a row all of whose keys score -inf has no softmax (NaN); a row that sees no key is 0; one that sees a finite score besides is finite"""
+    b = Batch(q_lens, kv_lens, Hkv, hd, 16, seed=hd, device=DEV, extra_width=1)
+    x = rnd(b.N, Hq * hd, seed=4).to(BF)
+    x.view(b.N, Hq, hd)[:, :, 0] = x.view(b.N, Hq, hd)[:, :, 0].abs() + 0.125
+    for some in (False, True):
+        kv0 = kv_lens[0]
+        for j in range(kv0 - 1 if some else kv0):                                   # all keys of the first slot, then all but its last
+            b.pages[b.row(0, j)][:Hkv * hd:hd] = -INF
+        if some:
+            b.pages[b.row(0, kv0 - 1)][:Hkv * hd:hd] = 0.5
+        got = ops.attention_paged(x, b.pages, b.table, b.cu_q, b.kv_len, Hq, Hkv, hd, causal=causal)
+        want = defined(b, x, Hq, causal)
+        q0 = q_lens[0]
+        hidden = max(q0 - kv0, 0) if causal else 0                                  # rows without a position
+        assert torch.isnan(want[hidden:q0]).any() == (not some or (causal and q0 > hidden + 1))
+        _, slack = attend(b, x, Hq, causal=causal)
+        same_kind(got, want, slack, f"some={some}")
+
+
+def test_attention_paged_slots_whose_pages_are_all_outside_the_pool_stay_zero():
+    for q, kv in ((1, 70), (1, 9000), (200, 300), (200, 4000)):
+        b = Batch([q], [kv], 2, 64, 64, device=DEV, holes=[(0, j, -1) for j in range(-(-kv // 64))])
+        b.pages.fill_(-INF)
+        out = ops.attention_paged(rnd(q, 4 * 64).to(BF), b.pages, b.table, b.cu_q, b.kv_len, 4, 2, 64)
+        assert (out == 0).all()

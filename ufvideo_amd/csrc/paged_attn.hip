@@ -1,6 +1,6 @@
 // Attention of a chunk of new tokens over a paged KV cache (see paged.h for the layout).
 //   o[r, h] = sum_j softmax_j(q[r, h] . k[j, g] * scale) v[j, g],  g = h / G,  G = Hq / Hkv,  over the keys j < kv_len[s] (causal: j <= the row's own position);
-// a row that sees no key gets zeros.  Keys that do not exist -- behind kv_len, in a page outside the pool -- are staged as zeros and their scores are -inf.
+// a row that sees no key gets zeros, one that sees keys of score -inf only NaN.  Keys that do not exist -- behind kv_len, in a page outside the pool -- are staged as zeros and their scores are -inf.
 //
 // The unit of work is a TILE of rows of one slot and one kv head, a row being a (token, q head of the group) pair: row r of a slot is token r / G, head g * G + r % G.  All G heads
 // that share a kv head sit in one tile, so that every key is fetched once for the group and a single token already fills G of the 32 columns of a matrix instruction.
@@ -258,6 +258,18 @@ __device__ __forceinline__ void paged_add_bad(const PagedAttn& a, const PagedTil
                 }
             }
     }
+}
+
+// A row without a finite score has the maximum -inf and no weight at all.  Its sum is 0 where it sees no key (the row is zeros), and this where it sees keys, all of score -inf: 0 times the
+// inverse, which is past 2^128, is the NaN of a row that has no softmax.  To a sum with a weight in it (at least about 1) this adds nothing.
+constexpr float NO_WEIGHT = 0x1p-149f;
+// behind a walk over the keys j0 .. j1 - 1
+template <int HDP>
+__device__ __forceinline__ void paged_no_weight(const PagedAttn& a, const PagedTile& w, int j0, int j1, PState<HDP>& st, int seen) {
+    if (!__any(st.m == -INFINITY)) return;
+    const int end = min(j1, w.len);
+    while (j0 < end && paged_row(a.t, w.s, j0) < 0) j0 += 16;                          // the first key that exists
+    if (st.m == -INFINITY && st.l == 0.f && j0 < min(seen, end)) st.l = NO_WEIGHT;
 }
 
 // zero the non-finite elements of a chunk of V; true if there was one
@@ -621,6 +633,7 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : HDP > 32 ? 2 : 4) void att
             else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                        // nothing is under way when the next item fills the ring
             __syncthreads();
         }
+        paged_no_weight<HDP>(a, w, t0 << 6, t1 << 6, st, seen);
         if ((int64_t)t1 * 64 > diag) {
             if (bad) dirty = 1;
             __syncthreads();
@@ -822,6 +835,7 @@ __global__ __launch_bounds__(NW * 64, HDP > 128 ? 1 : 2) void attn_paged_keys_k(
     }
     if (dirty)
         for (int t = t0 + wave; t < t1; t += NW) paged_add_bad<HDP>(a, w, max(max(diag, 0) & ~31, t << 5), min((t + 1) << 5, w.len), st, seen);
+    paged_no_weight<HDP>(a, w, t0 << 5, t1 << 5, st, seen);
     // ---- join the waves: (m, l) and O [row][HDP] of every wave through LDS, then every thread sums quads of the rows that exist
     const float l = st.l + __shfl_xor(st.l, 32, 64);
     if (h == 0) { wm[wave][l31] = st.m; wl[wave][l31] = l; }
