@@ -540,7 +540,7 @@ UFV_API int ufv_mask_loss_bwd(const float* x, const float* t, const float* coef,
  * memory and are read when the kernel runs: the launch arguments do not change from step to step, so a step can be recorded into a HIP graph.  Page ids are checked
  * against n_pages on the device: a key whose page id is outside is treated as absent, a row that has no page is not stored. */
 /* rotary positions with several axes (time, height, width): table f32 [N, hd] = cos | sin of positions[axis_of[i]][n] * inv_freq[i] (the layout of ufv_rope_table:
- * ufv_rope_kv_table, ufv_gemm_qkv_rope and the two entries below read it).  positions int64 [n_axes <= 4][N], pitch ld_pos; axis_of: hd/2 bytes in HOST memory, the axis
+ * ufv_rope_kv_table, ufv_gemm_qkv_rope and the two entries below read it).  positions int64 [n_axes <= 4][N], pitch ld_pos (0: one row for all axes); axis_of: hd/2 bytes in HOST memory, the axis
  * of every frequency pair.  The angle is formed and reduced in 64 bits (ufv_rope_table forms it in 32: its HF original does). */
 UFV_API int ufv_rope_axes_table(const float* inv_freq, const int64_t* positions, int64_t ld_pos, int n_axes, const uint8_t* axis_of, int N, int hd, float* table, void* stream);
 /* rotate-half RoPE of rows of `nheads` heads by a table: y (may be x) bf16 [N, ldy]; backward != 0: the transposed rotation (gradient of the forward one) */

@@ -142,3 +142,14 @@ def test_attention_paged_slots_whose_pages_are_all_outside_the_pool_stay_zero():
         b.pages.fill_(-INF)
         out = ops.attention_paged(rnd(q, 4 * 64).to(BF), b.pages, b.table, b.cu_q, b.kv_len, 4, 2, 64)
         assert (out == 0).all()
+
+
+# ---- strides that say nothing -----------------------------------------------------------------------------------------------------
+def test_rope_axes_table_of_one_set_of_positions_for_all_axes():
+    """text: the same positions on every axis, expanded, not copied"""
+    inv = (1.0 / (1e6 ** (torch.arange(0, 128, 2, dtype=torch.float32) / 128))).to(DEV)
+    for n in (1, 2, 300):
+        p = torch.arange(n, device=DEV) + 7
+        for axes in (1, 2, 3, 4):
+            amap = [i % axes for i in range(64)]
+            assert torch.equal(ops.rope_axes_table(inv, p.expand(axes, n), amap), ops.rope_axes_table(inv, p.expand(axes, n).contiguous(), amap))

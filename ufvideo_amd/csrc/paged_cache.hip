@@ -336,7 +336,7 @@ __global__ __launch_bounds__(256) void kv_pages_move_k(char* pool, int layers, i
 extern "C" int ufv_rope_axes_table(const float* inv_freq, const int64_t* positions, int64_t ld_pos, int n_axes, const uint8_t* axis_of, int N, int hd, float* table, void* stream) {
     UFV_REQUIRE(inv_freq && positions && axis_of && table && N > 0, "ufv_rope_axes_table: bad arguments");
     UFV_REQUIRE(hd > 0 && hd % 2 == 0 && hd <= 256, "ufv_rope_axes_table: head_dim must be even and at most 256 (%d)", hd);
-    UFV_REQUIRE(n_axes >= 1 && n_axes <= 4 && (n_axes == 1 || ld_pos >= N), "ufv_rope_axes_table: 1 to 4 axes, rows of at least N positions (%d axes, pitch %lld)", n_axes, (long long)ld_pos);
+    UFV_REQUIRE(n_axes >= 1 && n_axes <= 4 && (n_axes == 1 || ld_pos >= N || ld_pos == 0), "ufv_rope_axes_table: 1 to 4 axes, rows of at least N positions or one row for all (%d axes, pitch %lld)", n_axes, (long long)ld_pos);
     AxisMap m = {};
     for (int i = 0; i < hd / 2; ++i) {
         UFV_REQUIRE(axis_of[i] < n_axes, "ufv_rope_axes_table: pair %d names axis %d of %d", i, axis_of[i], n_axes);
