@@ -153,3 +153,37 @@ def test_rope_axes_table_of_one_set_of_positions_for_all_axes():
         for axes in (1, 2, 3, 4):
             amap = [i % axes for i in range(64)]
             assert torch.equal(ops.rope_axes_table(inv, p.expand(axes, n), amap), ops.rope_axes_table(inv, p.expand(axes, n).contiguous(), amap))
+
+
+def test_paged_views_of_one_entry():
+    """a single page out of larger ones, a table of one column, a single row of an odd pitch, a single slot, a single layer: the stride along an axis of one entry says nothing"""
+    Hq, Hkv, hd, page = 4, 2, 64, 16
+    big = rnd(3, 64, 2 * Hkv * hd, seed=1).to(BF)
+    one, same = big[1:2, :page], big[1:2, :page].contiguous()
+    assert one.stride(0) != page * one.stride(1)
+    column, dense = i32([[7, 0, 9]] * 2).t().contiguous().t()[:, 1:2], i32([[0], [0]])
+    assert column.stride() == (1, 2)
+    lens, cu = i32([9, 4]), i32([0, 1, 1])
+    wide = rnd(1, (Hq + 2 * Hkv) * hd + 3, seed=2).to(BF)
+    row = wide.as_strided((1, (Hq + 2 * Hkv) * hd), (wide.shape[1], 1))
+    assert row.stride(0) % 8
+    tab = rnd(1, hd, seed=3)
+    b = same.clone()
+    pool = big.clone()
+    view = pool[1:2, :page]
+    q1 = ops.rope_kv_paged(row, tab, Hq, Hkv, hd, view, column, cu, lens, q_out=torch.empty(1, Hq * hd + 1, device=DEV, dtype=BF))[:, :Hq * hd]
+    q2 = ops.rope_kv_paged(row.clone(memory_format=torch.contiguous_format), tab, Hq, Hkv, hd, b, dense, cu, lens)
+    assert torch.equal(q1, q2) and torch.equal(view, b) and torch.equal(pool[1, page:], big[1, page:]) and torch.equal(pool[::2], big[::2])
+    o1 = ops.attention_paged(q1, view, column, cu, lens, Hq, Hkv, hd)
+    assert torch.equal(o1, ops.attention_paged(q2.contiguous(), b, dense, cu, lens, Hq, Hkv, hd)) and o1.abs().max() > 0
+    assert torch.equal(ops.rope_rows_table(row, tab, 3, 2, hd, out=torch.empty(1, 2 * hd + 5, device=DEV, dtype=BF))[:, :2 * hd],
+                       ops.rope_rows_table(row[:, 3:].contiguous(), tab, 0, 2, hd, out=torch.empty(1, 2 * hd, device=DEV, dtype=BF)))
+    layers = rnd(4, 5, 64, 24, seed=5).to(BF)
+    few = layers[1:3, 2:3, :page]                                                     # one page a layer, out of larger ones
+    assert few.stride(1) != page * 24
+    keep = layers.clone()
+    ops.kv_pages_copy(few, i32([(0, 0, 3), (-1, 0, 2)]))
+    tables, held, refs = i32([[-1, -1], [0, -1]]), i32([0, 5]), i32([1])
+    assert ops.kv_pages_compact(few, tables, held, refs).tolist() == [1, 0] and torch.equal(layers, keep)
+    granted, cu_q, pairs = ops.kv_pages_extend(column, i32([1, 0]), i32([2]), i32([0, 1]), page)
+    assert granted.tolist() == [0, 0]

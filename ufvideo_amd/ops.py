@@ -934,19 +934,19 @@ def _vec(t, n, di, name):
 
 
 def _rows(t, n, cols, di, name):
-    """bf16 rows of at least `cols` elements (n of them; None: any number) -> (address, pitch)"""
+    """bf16 rows of at least `cols` elements (n of them; None: any number) -> (address, pitch; of a single row one that keeps 16-byte alignment: its stride says nothing)"""
     sh, st = t.shape, t.stride()
     if t.dtype is not _BF or t.get_device() != di or len(sh) != 2 or sh[1] < cols or st[1] != 1 or (n is not None and sh[0] != n):
         _bad(name, f"bf16 [{'N' if n is None else n}, >= {cols}] rows on cuda:{di}", t)
-    return t.data_ptr(), st[0]
+    return t.data_ptr(), st[0] if sh[0] > 1 else cols + 7 & -8
 
 
 def _paged_args(pages, block_table, cu_q, kv_len, Hkv, hd, di):
     sh, st, bs = pages.shape, pages.stride(), block_table.shape
-    if pages.dtype is not _BF or len(sh) != 3 or sh[2] < 2 * Hkv * hd or st[2] != 1 or st[0] != sh[1] * st[1]:
+    if pages.dtype is not _BF or len(sh) != 3 or sh[2] < 2 * Hkv * hd or st[2] != 1 or (st[0] != sh[1] * st[1] and sh[0] > 1):
         _bad("pages", f"bf16 [n_pages, page, >= {2 * Hkv * hd}] with all rows at one pitch", pages)
     S = kv_len.shape[0]
-    if block_table.dtype is not _I32 or block_table.get_device() != di or len(bs) != 2 or bs[0] != S or block_table.stride(1) != 1:
+    if block_table.dtype is not _I32 or block_table.get_device() != di or len(bs) != 2 or bs[0] != S or (block_table.stride(1) != 1 and bs[1] > 1):
         _bad("block_table", f"int32 [{S}, max_pages] on cuda:{di}", block_table)
     return (pages.data_ptr(), sh[0], sh[1], st[1], block_table.data_ptr(), block_table.stride(0) if S > 1 else bs[1], bs[1], _vec(cu_q, S + 1, di, "cu_q"), _vec(kv_len, S, di, "kv_len"), S)
 
@@ -1043,7 +1043,7 @@ def attention_paged(q, pages, block_table, cu_q, kv_len, Hq, Hkv, hd, scale=None
 
 def _table_args(block_table, kv_len, refs, page):
     di, bs, S = _gpu_index(block_table, "block_table"), block_table.shape, kv_len.shape[0]
-    if block_table.dtype is not _I32 or len(bs) != 2 or bs[0] != S or block_table.stride(1) != 1:
+    if block_table.dtype is not _I32 or len(bs) != 2 or bs[0] != S or (block_table.stride(1) != 1 and bs[1] > 1):
         _bad("block_table", f"int32 [{S}, max_pages]", block_table)
     P = refs.shape[0]
     return di, S, P, (block_table.data_ptr(), block_table.stride(0) if S > 1 else bs[1], bs[1], _vec(kv_len, S, di, "kv_len"), S, _vec(refs, P, di, "refs"), P, page)
@@ -1073,9 +1073,9 @@ def kv_pages_free(block_table, kv_len, refs, mask, page):
 
 def _pool_args(pool):
     di, sh, st = _gpu_index(pool, "pool"), pool.shape, pool.stride()
-    if pool.dtype is not _BF or len(sh) != 4 or st[3] != 1 or st[2] != sh[3] or st[1] != sh[2] * sh[3]:
+    if pool.dtype is not _BF or len(sh) != 4 or st[3] != 1 or st[2] != sh[3] or (st[1] != sh[2] * sh[3] and sh[1] > 1):
         _bad("pool", "bf16 [layers, n_pages, page, width] with contiguous layers", pool)
-    return di, pool.data_ptr(), sh[0], 2 * st[0], sh[1], sh[2], 2 * sh[3]
+    return di, pool.data_ptr(), sh[0], 2 * st[0] if sh[0] > 1 else 0, sh[1], sh[2], 2 * sh[3]
 
 
 def kv_pages_copy(pool, pairs):
