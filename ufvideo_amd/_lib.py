@@ -189,12 +189,10 @@ def load():
     lib.ufv_abi_version.argtypes = []
     if lib.ufv_abi_version() != ABI_VERSION:
         raise UfvError(f"{LIB_PATH} has ABI version {lib.ufv_abi_version()}, this binding was written for {ABI_VERSION}: rebuild (make)")
-    for name, args in SIGNATURES.items():
-        fn = getattr(lib, name)
-        fn.argtypes = args
-        fn.restype = _i
-    for name, (args, res) in SIZE_FUNCS.items():
-        fn = getattr(lib, name)
+    for name, (args, res) in {**{n: (a, _i) for n, a in SIGNATURES.items()}, **SIZE_FUNCS}.items():
+        fn = getattr(lib, name, None)
+        if fn is None:                       # entries are added without a new version: an older build of the same one
+            raise UfvError(f"{LIB_PATH} has no {name}, which this binding was written for: rebuild (make)")
         fn.argtypes = args
         fn.restype = res
     _lib = lib
