@@ -35,14 +35,23 @@ NSTAGE = 3                # tile j lives in stage j % 3 (NT tiles per pass, NT %
 NPIECE = 9                # DMA pieces per wave per tile (a wave loads the K tile or the V tile of its head)
 QPIECES = 9               # staging holds the rows of units 0 and 1 (64 x 144 B = 9 pieces); unit 2's fragments come straight from global memory
 UNIT_BYTES = 32 * PK      # 4608
-def _seq_arg():
-    for i, a in enumerate(sys.argv):
-        if a == "--seq":
-            return int(sys.argv[i + 1])
-        if a.startswith("--seq="):
-            return int(a[6:])
-    return 576
-SEQ = _seq_arg()
+def _options():
+    """(--seq, --simple); anything else is refused"""
+    seq, simple, args = "576", False, sys.argv[1:]
+    while args:
+        a = args.pop(0)
+        if a == "--simple":
+            simple = True
+        elif a.startswith("--seq="):
+            seq = a[6:]
+        elif a == "--seq" and args:
+            seq = args.pop(0)
+        else:
+            seq = ""
+        if not seq.isdigit():
+            sys.exit(f"{a}: usage: gen_attn_p2.py [--seq S] [--simple]")
+    return int(seq), simple
+SEQ, SIMPLE = _options()
 NT = (SEQ + 63) // 64     # key tiles per pass (9 at S = 576, 12 at S = 729)
 NPASS = (SEQ + 191) // 192    # passes of 96 query rows per wave (3 / 4)
 REM = SEQ - 64 * (NT - 1)     # keys of the last tile that exist (64: nothing to mask)
@@ -607,7 +616,7 @@ def build(simple=False):
 
 
 def main():
-    simple = "--simple" in sys.argv
+    simple = SIMPLE
     lines = build(simple)
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     sfx = "" if SEQ == 576 else f"_s{SEQ}"              # file and macro names of the other sequence lengths carry the length
