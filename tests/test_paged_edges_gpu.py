@@ -6,7 +6,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 from paged_ref import Batch, attend  # noqa: E402
-from ufvideo_amd import ops  # noqa: E402
+from ufvideo_amd import _lib, ops  # noqa: E402
 
 DEV = "cuda"
 BF = torch.bfloat16
@@ -187,3 +187,19 @@ def test_paged_views_of_one_entry():
     assert ops.kv_pages_compact(few, tables, held, refs).tolist() == [1, 0] and torch.equal(layers, keep)
     granted, cu_q, pairs = ops.kv_pages_extend(column, i32([1, 0]), i32([2]), i32([0, 1]), page)
     assert granted.tolist() == [0, 0]
+
+
+def test_paged_ops_refuse_heads_that_do_not_exist():
+    """no heads, no head_dim, negative ones: an error of the operators' own, whatever is computed from them on the way"""
+    b = Batch([2], [20], 2, 64, 16, device=DEV)
+    q, tab = rnd(2, 512).to(BF), rnd(2, 64)
+    for Hq, Hkv, hd in ((4, 2, 0), (4, 2, -8), (0, 2, 64), (-4, 2, 64), (4, 0, 64), (4, -2, 64), (2, 4, 64)):
+        with pytest.raises(_lib.UfvError):
+            ops.attention_paged(q, b.pages, b.table, b.cu_q, b.kv_len, Hq, Hkv, hd)
+        with pytest.raises(_lib.UfvError):
+            ops.attention_paged(q, b.pages, b.table, b.cu_q, b.kv_len, Hq, Hkv, hd, out=torch.empty_like(q))
+        with pytest.raises(_lib.UfvError):
+            ops.rope_kv_paged(q, tab if hd == 64 else rnd(2, max(hd, 0)), Hq, Hkv, hd, b.pages, b.table, b.cu_q, b.kv_len)
+    for heads, hd in ((0, 64), (-1, 64), (2, 0), (2, -4)):
+        with pytest.raises(_lib.UfvError):
+            ops.rope_rows_table(q, rnd(2, max(hd, 0)), 0, heads, hd)

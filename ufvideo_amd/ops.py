@@ -941,7 +941,9 @@ def _rows(t, n, cols, di, name):
     return t.data_ptr(), st[0] if sh[0] > 1 else cols + 7 & -8
 
 
-def _paged_args(pages, block_table, cu_q, kv_len, Hkv, hd, di):
+def _paged_args(pages, block_table, cu_q, kv_len, Hq, Hkv, hd, di):
+    if Hq < 1 or Hkv < 1 or hd < 1:
+        raise _lib.UfvError(f"heads and head_dim must be positive ({Hq} q heads on {Hkv} kv heads of {hd})")
     sh, st, bs = pages.shape, pages.stride(), block_table.shape
     if pages.dtype is not _BF or len(sh) != 3 or sh[2] < 2 * Hkv * hd or st[2] != 1 or (st[0] != sh[1] * st[1] and sh[0] > 1):
         _bad("pages", f"bf16 [n_pages, page, >= {2 * Hkv * hd}] with all rows at one pitch", pages)
@@ -1009,7 +1011,7 @@ def rope_kv_paged(qkv, table, Hq, Hkv, hd, pages, block_table, cu_q, kv_len, q_o
     """RoPE of the packed new tokens' q and k heads and append of their k / v rows to the pages (the paged form of `rope_kv`).  qkv bf16 [N, (Hq + 2 Hkv)*hd]; kv_len
     counts the new tokens already (kv_pages_extend).  Returns the rotated q: the q columns of qkv, or q_out bf16 [N, Hq*hd].  Rows behind cu_q[S] stay as they are."""
     di = _gpu_index(pages, "pages")
-    pa = _paged_args(pages, block_table, cu_q, kv_len, Hkv, hd, di)
+    pa = _paged_args(pages, block_table, cu_q, kv_len, Hq, Hkv, hd, di)
     N = qkv.shape[0]
     src, ldx = _rows(qkv, None, (Hq + 2 * Hkv) * hd, di, "qkv")
     dst, ldo = (src, ldx) if q_out is None else _rows(q_out, N, Hq * hd, di, "q_out")
@@ -1028,7 +1030,7 @@ def attention_paged(q, pages, block_table, cu_q, kv_len, Hq, Hkv, hd, scale=None
     """Attention of the packed new tokens (q bf16 [N, Hq*hd], slot s has rows cu_q[s] .. cu_q[s+1]) over their slots' cached tokens: a chunk of a prompt, a decode step of
     many conversations, or both in one batch.  causal: a row sees the cached tokens up to its own.  A row that sees none gets zeros, rows behind cu_q[S] stay as they are."""
     di = _gpu_index(pages, "pages")
-    pa = _paged_args(pages, block_table, cu_q, kv_len, Hkv, hd, di)
+    pa = _paged_args(pages, block_table, cu_q, kv_len, Hq, Hkv, hd, di)
     N = q.shape[0]
     src, ldq = _rows(q, None, Hq * hd, di, "q")
     if out is None:
