@@ -550,7 +550,7 @@ UFV_API int ufv_rope_rows_table(const void* x, int64_t ldx, void* y, int64_t ldy
 UFV_API int ufv_rope_kv_paged(const void* qkv, int64_t ldqkv, void* q_out, int64_t ldq, int N, int Hq, int Hkv, int hd, const float* table, void* pages, int n_pages, int page,
                               int64_t ldkv, const int32_t* block_table, int64_t ld_table, int max_pages, const int32_t* cu_q, const int32_t* kv_len, int S, void* stream);
 /* o[n] = softmax(q k^T * scale) v of every packed row over its slot's cached tokens (causal: up to the row's own), GQA, fp32 softmax; a row that sees no key gets zeros,
- * a row all of whose keys score -inf NaN.
+ * a row all of whose keys score -inf NaN.  64 times the sum of |v| over a row's keys has to stay below 2^128 (the weights are divided by their sum at the end).
  * q, o bf16, head h at column h*hd; hd a multiple of 8 up to 256; scale positive and finite; ldkv below 2^24.  cu_q must ascend.  ws, 16-byte aligned, of any content: ufv_attention_paged_ws_bytes(N, S, Hq, Hkv, hd, max_pages * page) bytes (may be 0), not shared by
  * calls that can run at the same time. */
 UFV_API int64_t ufv_attention_paged_ws_bytes(int N, int S, int Hq, int Hkv, int hd, int max_keys);
@@ -563,7 +563,7 @@ UFV_API int ufv_kv_pages_fork(int32_t* block_table, int64_t ld_table, int max_pa
 /* extend: room for n_new[s] further tokens of every slot, kv_len[s] += n_new[s].  Pages are the lowest free ids in slot order; a partly filled last page that is shared
  * when the call starts is replaced by a page of its own (pairs[s] = (old, new, rows to copy), else (-1, -1, 0): ufv_kv_pages_copy moves the rows).  A slot whose share
  * reaches past the free pages (counting the shares of all slots before it) or past its table row gets nothing; new tokens that fit its own last page need none.
- * granted[s] = tokens granted, cu_q int32 [S+1] = their prefix sum.  max_pages <= 2^20. */
+ * granted[s] = tokens granted, cu_q int32 [S+1] = their prefix sum (below 2^31 in all).  max_pages <= 2^20. */
 UFV_API int64_t ufv_kv_pages_extend_ws_bytes(int S, int n_pages);
 UFV_API int ufv_kv_pages_extend(int32_t* block_table, int64_t ld_table, int max_pages, int32_t* kv_len, int S, int32_t* refs, int n_pages, int page, const int32_t* n_new, int32_t* granted,
                                 int32_t* cu_q, int32_t* pairs, void* ws, int64_t ws_bytes, void* stream);

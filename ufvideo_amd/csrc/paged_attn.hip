@@ -8,10 +8,11 @@
 // Both kernels compute S^T = K Q^T with v_mfma_f32_32x32x16_bf16 (a lane owns one row of the tile: its column of S^T), keep the running maximum and sum of the softmax in
 // 32 bits (log2 domain), and use the exponentiated tile, rounded to bf16, directly as the B operand of O^T += V^T P^T.  The rounding of P is the one step below 32 bits between
 // the inputs and the output: the matrix instruction takes bf16 operands; the row sum is taken of the unrounded values.  V^T fragments come from row-major V rows in LDS by the transposing read.
-//   attn_paged_tile_k   the waves of a block share 64-key tiles and split the ROWS: chunks of many rows, bound by the matrix unit.  28 / 4 heads of 128: 2399 tokens over 20011 in 660 us
-//                       (0.98 PF/s with its join), 8192 causal tokens 600 us, 16 questions of 9 .. 83 tokens behind 2304 shared ones 58 us (0.43 PF/s: 13 steps a block, then the join)
-//   attn_paged_keys_k   the waves of a block share up to 32 rows and split the KEYS: a few new tokens over a long cache, bound by the bytes of the cache.  48 slots of 714 .. 5825 tokens
-//                       57 us (5.0 TB/s; a large read reaches 6.1), one of 31999 24 us (2.8 TB/s: 4 us until the first keys are asked for, 5 us for the join)
+//   attn_paged_tile_k   the waves of a block share 64-key tiles and split the ROWS: chunks of many rows, bound by the matrix unit.  28 / 4 heads of 128: 2399 tokens over 20011 in 690 us
+//                       (0.94 PF/s with its join; 650 .. 725 from run to run), 8192 causal tokens 575 us, 16 questions of 12 .. 82 tokens behind 2304 shared ones 49 us and 9 for the join
+//                       (0.44 PF/s: 14 steps a block of 2.2 us, 11 of starts and ends, 6 until the longest block is done)
+//   attn_paged_keys_k   the waves of a block share up to 32 rows and split the KEYS: a few new tokens over a long cache, bound by the bytes of the cache.  48 slots of 792 .. 6045 tokens
+//                       73 us and 5 for the join (4.4 TB/s; a large read reaches 6.1), one of 31999 17 us and 6 (2.8 TB/s: 4 us until the first keys are asked for)
 // The work is cut over the keys for the 256 CUs; the parts leave (max, sum, un-normalised O) in 32 bits in the workspace and attn_paged_join_k adds them in order.
 #include "paged.h"
 
@@ -126,12 +127,12 @@ struct PState {
 
 // NH half tiles of 32 keys in LDS (K rows at kb, V rows at vb) against 32 rows: S^T, running softmax, O^T.  hide: key j of the step counts for the lane's row iff j < vis and, in groups of 16
 // keys, iff its bit of `groups` is set.
-// at_qk(i, n, next) runs behind the i-th of the n products of S^T: the loads of a later step (memory -> LDS at `next`) go there, a few at a time -- issued in one go they hold the wave for
-// 1300 of the 4500 cycles of a step (the memory pipe takes one 1 KB load in 16 cycles), behind the products they cost little.  kb, vb, next do not overlap (__restrict__ lets the compiler
+// at_qk(i, n, next) runs behind the i-th of the n products of S^T: the loads of a later step (memory -> LDS at `next`) go there, a few at a time -- issued in one go they hold the wave
+// (the memory pipe takes one 1 KB load in 16 cycles), behind the products they cost little.  kb, vb, next do not overlap (__restrict__ lets the compiler
 // keep the loads in flight across the reads: who issues them waits for them before the barrier that publishes them).
-// A step of 64 keys at head_dim 128 is 1024 cycles of the matrix unit, two waves a SIMD: 2048.  16384 rows over 8192 keys run at 1.05 PF/s (4400 cycles a step); without the LDS reads they would
-// take 5 % less, without the exponentials 7 %, without the loads 7 %, without all three 21 % -- no one of them bounds it, and then the clock falls: the products alone reach 1.26 PF/s, a large
-// library product 1.42.  Tried and slower: the exponentials between the products of the next step's S^T (8 %; the maximum between those of O^T), 64 rows a wave (30 %), waves in two groups
+// A step of 64 keys at head_dim 128 is 1024 cycles of the matrix unit, two waves a SIMD: 2048.  16384 tokens over 8192 keys (28 / 4 heads) run at 1.02 PF/s, 4400 cycles a step; without the LDS reads they
+// would take 7 % less, without the exponentials 8 %, without the loads 7 %, without all three 23 % -- no one of them bounds it, and then the clock falls: the products alone reach 1.26 PF/s, a
+// large library product 1.41.  Tried and slower: the exponentials between the products of the next step's S^T (8 %; the maximum between those of O^T), 64 rows a wave (30 %), waves in two groups
 // half a step apart (4 %).
 template <int HDP, int NH, class FQ>
 __device__ __forceinline__ void paged_step(const char* __restrict__ kb, const char* __restrict__ vb, char* __restrict__ next, const bf16x8 (&qf)[HDP / 16], PState<HDP>& st, float sl2, bool hide, int vis,
@@ -179,7 +180,8 @@ __device__ __forceinline__ void paged_step(const char* __restrict__ kb, const ch
 #pragma unroll
         for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, s[hh][r]);
     tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64)) * sl2;
-    // the rescale of O waits until the maximum has grown by 2^6: until then the exponentials stay below 2^6 and nothing is lost
+    // the rescale of O waits until the maximum has grown by 2^6: until then the exponentials stay below 2^6.  No bits are lost, but range is: O before the division is up to 64 sum |v| (a sum of
+    // weights up to 1 would be up to sum |v|) and has to stay below 2^128
     if (__any(tmax > st.m + 6.0f)) {
         const float mnew = fmaxf(st.m, tmax);
         const float alpha = mnew == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.m - mnew);
@@ -971,7 +973,8 @@ struct Plan {
     int64_t ws;             // bytes
 };
 
-// N, S: packed rows and slots; the lengths are on the device, the choice is made from the sizes alone.  A slot has N / S rows on average.
+// N, S: packed rows and slots; the lengths are on the device, the choice is made from the sizes alone: N / S rows a slot, as if all of them were as busy (the figures below are of such batches).  A
+// batch of one long chunk in a table of idle slots is right, but may run through tiles of 32 rows that each fetch the chunk's whole cache.
 Plan make_plan(int N, int S, int Hq, int Hkv, int hd, int max_keys) {
     const int G = Hq / Hkv, hdp = hd > 128 ? 256 : (hd + 31) / 32 * 32, used = S < N ? S : N;
     const int64_t rows = (int64_t)N * G;

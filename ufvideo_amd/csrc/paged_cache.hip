@@ -9,7 +9,7 @@ namespace {
 // ---------------------------------------------------------------------------------------------------------------------------------
 // cos | sin of p[a(i)][n] * inv_freq[i]: rotary positions with several axes.  Frequency pair i turns with the position on ITS axis (time, height, width:
 // a(i) comes from the host, two bits per pair).  The angle is formed and reduced to a turn in 64 bits -- at position 10^6 a 32-bit product is off by up to
-// 0.03 rad, 64 bits leave 10^-10 -- and the functions of the reduced angle are 32-bit (1-2 ulp).  A thread a pair: 2399 rows of 64 pairs 3.2 us (launch and latency), 16383 rows 6.0 us.
+// 0.03 rad, 64 bits leave 10^-10 -- and the functions of the reduced angle are 32-bit (1-2 ulp).  A thread a pair: 2399 rows of 64 pairs 3.2 us (launch and latency), 16383 rows 6.1 us.
 // ---------------------------------------------------------------------------------------------------------------------------------
 struct AxisMap { uint32_t w[8]; };      // pair i: bits 2 (i & 15) of word i >> 4; by value: no device copy of the map exists
 
@@ -47,7 +47,7 @@ __device__ __forceinline__ void rope_chunk8(const bf16x8 a, const bf16x8 b, cons
 }
 
 // y = rotated x, rows of nheads heads.  Thread = (row, head, chunk of 8 pairs): two 16-byte loads and stores, the table row from the caches for all heads but one.  Bound by HBM: 16383 rows of
-// 32 heads of 128 41 us = 6.6 TB/s, 2399 rows 7.2 us.
+// 32 heads of 128 41 us = 6.8 TB/s, 2399 rows 6.9 us.
 __global__ __launch_bounds__(256) void rope_rows_table_k(const bf16* x, int64_t ldx, bf16* y, int64_t ldy, int N, int nheads, int hd, const float* __restrict__ tab, float sg) {
     const int half = hd >> 1, cpr = half >> 3;
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(256) void rope_rows_table_scalar_k(const bf16* x, i
 }
 
 // q_out = rotated q, cache row = [rotated k | v] of every packed row.  Block = one row: its slot, position and page are block-uniform; thread = (head, chunk of 8 pairs).  Bound by HBM: 6449 rows
-// of 28 + 2 x 4 heads of 128 20 us = 6 TB/s; one row 2.5 us.
+// of 28 + 2 x 4 heads of 128 20.6 us = 5.9 TB/s; one row 2.4 us.
 __global__ void rope_kv_paged_k(const bf16* qkv, int64_t ldqkv, bf16* q_out, int64_t ldq, int Hq, int Hkv, int hd, const float* __restrict__ tab, bf16* __restrict__ pages,
                                 int64_t ldkv, PagedTable t) {
     const int n = blockIdx.x;
@@ -138,7 +138,7 @@ __device__ __forceinline__ int block_scan(int v, int* red, int& total) {
     return before + x - v;
 }
 
-// slot s becomes another owner of every page of slot parent[s] (no page is copied; latency: 24 slots 2.9 us).  A slot that holds tokens is no child, a slot that is named a child is no parent:
+// slot s becomes another owner of every page of slot parent[s] (no page is copied; latency: 24 slots 3 us).  A slot that holds tokens is no child, a slot that is named a child is no parent:
 // no block reads what another one writes, whatever the vector says.
 __global__ __launch_bounds__(256) void kv_pages_fork_k(int* table, int64_t ld, int width, int* kv_len, int* refs, int n_pages, const int* __restrict__ parent, int S, int sh) {
     const int s = blockIdx.x, p = parent[s];
@@ -168,7 +168,7 @@ __global__ __launch_bounds__(256) void kv_pages_free_k(int* table, int64_t ld, i
     if (threadIdx.x == 0) kv_len[s] = 0;
 }
 
-// Room for n_new[s] further tokens of every slot, one block of 1024 threads (a chain of scans and dependent loads, latency: 24 slots on 93 pages 7 us):
+// Room for n_new[s] further tokens of every slot, one block of 1024 threads (a chain of scans and dependent loads, latency: 24 slots on 93 pages 7.8 us):
 //  A  what every slot needs: new pages at its end, and a page of its own in place of a partly filled last page that it shares (copy on write); prefix sum over the slots
 //  B  the lowest free page ids, as many as are needed (the scan of refs stops there)
 //  C  slot s takes pages [off, off + need) of that list, one wave per slot; a slot whose share reaches past the free pages, or past its table row, gets nothing
@@ -284,7 +284,7 @@ __global__ __launch_bounds__(1024) void kv_pages_plan_k(int* refs, int n_pages, 
     if (tid == 0) { counts[0] = live; counts[1] = movers; }
 }
 
-// 16 KB of one page: 256 threads x 4 x 16 bytes, all four loads before the first store (copies of 82 MB in 14.6 us = 5.6 TB/s, moves of 228 MB in 37 = 6.1: bound by HBM)
+// 16 KB of one page: 256 threads x 4 x 16 bytes, all four loads before the first store (copies of 82 MB in 15 us = 5.4 TB/s, moves of 228 MB in 37 = 6.1: bound by HBM)
 __device__ __forceinline__ void copy_piece(const char* __restrict__ src, char* __restrict__ dst, int64_t bytes, int64_t at) {
     typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
     u32x4 v[4];
