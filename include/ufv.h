@@ -557,7 +557,7 @@ UFV_API int64_t ufv_attention_paged_ws_bytes(int N, int S, int Hq, int Hkv, int 
 UFV_API int ufv_attention_paged(const void* q, int64_t ldq, void* o, int64_t ldo, int N, int Hq, int Hkv, int hd, const void* pages, int n_pages, int page, int64_t ldkv,
                                 const int32_t* block_table, int64_t ld_table, int max_pages, const int32_t* cu_q, const int32_t* kv_len, int S, float scale, int causal, void* ws,
                                 int64_t ws_bytes, void* stream);
-/* page management.  refs int32 [n_pages]: how many table entries name a page, 0 = free.  Requests are dense vectors over the slots (int32 [S]).
+/* page management.  At most 2^30 pages and 2^29 slots.  refs int32 [n_pages]: how many table entries name a page, 0 = free.  Requests are dense vectors over the slots (int32 [S]).
  * fork: slot s with parent[s] >= 0 becomes another owner of the parent's pages (nothing is copied).  Ignored where s holds tokens or the parent is named a child itself. */
 UFV_API int ufv_kv_pages_fork(int32_t* block_table, int64_t ld_table, int max_pages, int32_t* kv_len, int S, int32_t* refs, int n_pages, int page, const int32_t* parent, void* stream);
 /* extend: room for n_new[s] further tokens of every slot, kv_len[s] += n_new[s].  Pages are the lowest free ids in slot order; a partly filled last page that is shared

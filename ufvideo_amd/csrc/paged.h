@@ -53,6 +53,7 @@ static inline int paged_log2(int page) {
 #define UFV_REQUIRE_PAGED(name, pages, n_pages, page, ldkv, table, ld_table, max_pages, cu_q, kv_len, S)                                              \
     UFV_REQUIRE((pages) && (table) && (cu_q) && (kv_len) && (n_pages) > 0 && (max_pages) > 0 && (S) > 0 && (ld_table) >= (max_pages),                 \
                 name ": bad arguments (%d pages, %d slots, table %d of pitch %lld)", n_pages, S, max_pages, (long long)(ld_table));                   \
+    UFV_REQUIRE((S) <= 1 << 29, name ": more than 2^29 slots (%d)", S);                                                                               \
     UFV_REQUIRE(paged_log2(page) > 0, name ": the page size must be a power of two from 16 to 32768 (%d)", page);                                     \
     UFV_REQUIRE((uintptr_t)(pages) % 16 == 0 && (ldkv) % 8 == 0, name ": cache rows must be 16-byte aligned (pitch %lld)", (long long)(ldkv));        \
     UFV_REQUIRE(((int64_t)(max_pages) << paged_log2(page)) <= 0x7fffffff - 65536, name ": a table row names more than 2^31 tokens (%d pages of %d)", max_pages, page)

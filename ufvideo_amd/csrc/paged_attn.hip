@@ -1052,7 +1052,8 @@ extern "C" int ufv_attention_paged(const void* q, int64_t ldq, void* o, int64_t 
     UFV_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)o % 16 == 0 && ldq % 8 == 0 && ldo % 8 == 0, "ufv_attention_paged: rows must be 16-byte aligned (pitches %lld, %lld)", (long long)ldq,
                 (long long)ldo);
     UFV_REQUIRE(ldkv >= 2 * (int64_t)Hkv * hd && ldkv < 1 << 24 && (N == 1 || (ldq >= (int64_t)Hq * hd && ldo >= (int64_t)Hq * hd)), "ufv_attention_paged: a row pitch is out of range");
-    UFV_REQUIRE((int64_t)N * Hq < 0x7fffffff && S <= 65536, "ufv_attention_paged: too many rows or slots (N=%d S=%d)", N, S);
+    // (token, head) rows and those of a last tile's width behind them, columns of a row: 31 bits
+    UFV_REQUIRE((int64_t)N * Hq <= 0x7fffffff - 65536 && (int64_t)Hq * hd < 0x7fffffff && S <= 65536, "ufv_attention_paged: too many rows, columns or slots (N=%d, %d heads of %d, S=%d)", N, Hq, hd, S);
     const Plan p = make_plan(N, S, Hq, Hkv, hd, max_pages << paged_log2(page));
     UFV_REQUIRE(((int64_t)p.tiles + 2 * p.target) * Hkv < 0x7fffffff && Hkv < 65536, "ufv_attention_paged: too many row tiles (N=%d S=%d)", N, S);
     UFV_REQUIRE(p.ws == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= p.ws), "ufv_attention_paged: a 16-byte aligned workspace of %lld bytes is needed (%lld given)", (long long)p.ws,

@@ -351,6 +351,7 @@ extern "C" int ufv_rope_axes_table(const float* inv_freq, const int64_t* positio
 extern "C" int ufv_rope_rows_table(const void* x, int64_t ldx, void* y, int64_t ldy, int N, int nheads, int hd, const float* table, int backward, void* stream) {
     UFV_REQUIRE(x && y && table && N > 0 && nheads > 0 && hd > 0 && hd % 2 == 0, "ufv_rope_rows_table: bad arguments (N=%d heads=%d hd=%d)", N, nheads, hd);
     UFV_REQUIRE(N == 1 || (ldx >= (int64_t)nheads * hd && ldy >= (int64_t)nheads * hd), "ufv_rope_rows_table: row pitch below %d heads of %d", nheads, hd);
+    UFV_REQUIRE((int64_t)nheads * hd < 0x7fffffff, "ufv_rope_rows_table: rows of more than 2^31 columns (%d heads of %d)", nheads, hd);
     const float sg = backward ? -1.f : 1.f;
     const bool vec = hd % 16 == 0 && ldx % 8 == 0 && ldy % 8 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)y % 16 == 0 && (uintptr_t)table % 16 == 0;
     const int64_t total = (int64_t)N * nheads * (vec ? hd / 16 : hd / 2);
@@ -369,6 +370,7 @@ extern "C" int ufv_rope_kv_paged(const void* qkv, int64_t ldqkv, void* q_out, in
     UFV_REQUIRE((uintptr_t)qkv % 16 == 0 && (uintptr_t)q_out % 16 == 0 && (uintptr_t)table % 16 == 0 && ldqkv % 8 == 0 && ldq % 8 == 0,
                 "ufv_rope_kv_paged: rows must be 16-byte aligned (pitches %lld, %lld)", (long long)ldqkv, (long long)ldq);
     UFV_REQUIRE(ldkv >= 2 * (int64_t)Hkv * hd && (N == 1 || (ldqkv >= (int64_t)(Hq + 2 * Hkv) * hd && ldq >= (int64_t)Hq * hd)), "ufv_rope_kv_paged: a row pitch is too small");
+    UFV_REQUIRE(((int64_t)Hq + 2 * (int64_t)Hkv) * hd < 0x7fffffff, "ufv_rope_kv_paged: rows of more than 2^31 columns (heads %d/%d of %d)", Hq, Hkv, hd);
     PagedTable t{block_table, ld_table, max_pages, cu_q, kv_len, S, n_pages, paged_log2(page)};
     const int items = (Hq + 2 * Hkv) * (hd / 16), threads = items < 512 ? (items + 63) / 64 * 64 : 512;
     hipLaunchKernelGGL(rope_kv_paged_k, dim3(N), dim3(threads), 0, ST(stream), (const bf16*)qkv, ldqkv, (bf16*)q_out, ldq, Hq, Hkv, hd, table, (bf16*)pages, ldkv, t);
@@ -376,9 +378,11 @@ extern "C" int ufv_rope_kv_paged(const void* qkv, int64_t ldqkv, void* q_out, in
     return UFV_OK;
 }
 
+// (2^30 pages, 2^29 slots: the loops over them and three entries a slot stay within 31 bits)
 #define UFV_REQUIRE_TABLE(name)                                                                                                                   \
     UFV_REQUIRE(block_table && kv_len && refs && max_pages > 0 && S > 0 && n_pages > 0 && ld_table >= max_pages,                                 \
                 name ": bad arguments (%d slots, %d pages, table %d of pitch %lld)", S, n_pages, max_pages, (long long)ld_table);                 \
+    UFV_REQUIRE(n_pages <= 1 << 30 && S <= 1 << 29, name ": more than 2^30 pages or 2^29 slots (%d, %d)", n_pages, S);                            \
     UFV_REQUIRE(paged_log2(page) > 0, name ": the page size must be a power of two from 16 to 32768 (%d)", page);                                 \
     UFV_REQUIRE(((int64_t)max_pages << paged_log2(page)) <= 0x7fffffff - 65536, name ": a table row names more than 2^31 tokens (%d pages of %d)", max_pages, page)
 
