@@ -203,3 +203,23 @@ def test_paged_ops_refuse_heads_that_do_not_exist():
     for heads, hd in ((0, 64), (-1, 64), (2, 0), (2, -4)):
         with pytest.raises(_lib.UfvError):
             ops.rope_rows_table(q, rnd(2, max(hd, 0)), 0, heads, hd)
+
+
+@pytest.mark.parametrize("Hq,Hkv,hd", [(4, 2, 128), (4, 2, 72), (2, 1, 256)])
+@pytest.mark.parametrize("q,kv", [(3, 50), (40, 300), (150, 1517), (300, 300)])
+def test_attention_paged_an_infinite_v_of_weight_nothing_is_nan(Hq, Hkv, hd, q, kv):
+    """a key whose score is -inf and whose V holds infinities: 0 times them is NaN in their columns, before the new tokens and among them; the other columns go on without the key"""
+    b = Batch([q], [kv], Hkv, hd, 16, seed=hd, device=DEV)
+    x = rnd(b.N, Hq * hd, seed=q).to(BF)
+    x.view(q, Hq, hd)[:, :, 2] = x.view(q, Hq, hd)[:, :, 2].abs() + 0.125
+    clean, first = b.pages.clone(), kv - q
+    for at in sorted({first // 64 * 64, max(first - 1, 1), first + 1, kv - 1}):
+        if at == 0:                                                               # the only key of the first row: that row has no softmax
+            continue
+        b.pages.copy_(clean)
+        b.pages[b.row(0, at)][(Hkv - 1) * hd + 2] = -INF
+        b.pages[b.row(0, at)][(2 * Hkv - 1) * hd + 4], b.pages[b.row(0, at)][2 * Hkv * hd - 1] = INF, -INF
+        got = ops.attention_paged(x, b.pages, b.table, b.cu_q, b.kv_len, Hq, Hkv, hd)
+        want, slack = attend(b, x, Hq)
+        assert torch.isnan(want).any(0).sum() == 2 * (Hq // Hkv)
+        same_kind(got, want, slack, f"key {at} of {kv}, {q} new")

@@ -235,9 +235,22 @@ __device__ __forceinline__ void paged_step(const char* __restrict__ kb, const ch
     st.l += sum;
 }
 
+// zero the non-finite elements of a chunk; true if there was one
+__device__ __forceinline__ bool paged_clean(u32x4& v) {
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bool lo = (v[i] & 0x7f80u) == 0x7f80u, hi = (v[i] & 0x7f800000u) == 0x7f800000u;
+        v[i] &= (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0x0000ffffu : 0xffffffffu);
+        any |= lo | hi;
+    }
+    return any;
+}
+
 // A key that a row does not see must not reach it even when its V row holds Inf or NaN (0 * Inf in the matrix product): among the new tokens of a causal chunk -- the only keys
 // that some rows see and others do not -- such elements are staged as zeros, and if there was one, they are added after the walk to the rows that see them (keys j0 .. j1 - 1;
-// p > 0 times Inf or NaN is Inf or NaN).  Whole steps are cleaned, so the range begins at the first key of the step that holds the first new token, not at that token.
+// p > 0 times Inf or NaN is Inf or NaN; a K row with such an element has no finite score, so p is 0 or NaN and the product NaN).  Whole steps are cleaned, so the range begins at the first
+// key of the step that holds the first new token, not at that token.
 template <int HDP>
 __device__ __forceinline__ void paged_add_bad(const PagedAttn& a, const PagedTile& w, int j0, int j1, PState<HDP>& st, int seen) {
     int h = (threadIdx.x & 63) >> 5;
@@ -245,7 +258,11 @@ __device__ __forceinline__ void paged_add_bad(const PagedAttn& a, const PagedTil
     for (int j = j0; j < j1; ++j) {
         const int64_t at = paged_row(a.t, w.s, j);
         if (at < 0) continue;
-        const bf16* v = a.pages + at * a.ldkv + (a.Hkv + w.g) * a.hd;
+        const bf16 *k = a.pages + at * a.ldkv + w.g * a.hd, *v = k + a.Hkv * a.hd;
+        const int lane = threadIdx.x & 63;
+        u32x4 kc = {0, 0, 0, 0};
+        if (lane * 8 < a.hd) kc = *reinterpret_cast<const u32x4*>(k + lane * 8);
+        const bool nan = __any(paged_clean(kc));
 #pragma unroll
         for (int dt = 0; dt < HDP / 32; ++dt)
 #pragma unroll
@@ -256,7 +273,7 @@ __device__ __forceinline__ void paged_add_bad(const PagedAttn& a, const PagedTil
                     const bf16x4 x = *reinterpret_cast<const bf16x4*>(v + d);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (!(fabsf((float)x[e]) < INFINITY) && j < seen) st.o[dt][4 * g4 + e] += (float)x[e];
+                        if (!(fabsf((float)x[e]) < INFINITY) && j < seen) st.o[dt][4 * g4 + e] += nan ? __builtin_nanf("") : (float)x[e];
                 }
             }
     }
@@ -272,18 +289,6 @@ __device__ __forceinline__ void paged_no_weight(const PagedAttn& a, const PagedT
     const int end = min(j1, w.len);
     while (j0 < end && paged_row(a.t, w.s, j0) < 0) j0 += 16;                          // the first key that exists
     if (st.m == -INFINITY && st.l == 0.f && j0 < min(seen, end)) st.l = NO_WEIGHT;
-}
-
-// zero the non-finite elements of a chunk of V; true if there was one
-__device__ __forceinline__ bool paged_clean(u32x4& v) {
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const bool lo = (v[i] & 0x7f80u) == 0x7f80u, hi = (v[i] & 0x7f800000u) == 0x7f800000u;
-        v[i] &= (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0x0000ffffu : 0xffffffffu);
-        any |= lo | hi;
-    }
-    return any;
 }
 
 // The lane's rows of the tile as B operands (lane: row l31 of the group, dims 16 ks + 8 h ..), and what they see.  Rows behind the tile's last take the last one's q; they are not stored.
